@@ -150,9 +150,9 @@ def plain_codes(x):
 
 
 def activation(g, act):
-    if act == "silu":
-        return g / (1.0 + torch.exp(-g))
-    return 0.5 * g * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * (g + 0.044715 * g * g * g)))
+    """SiLU, or GELU in its tanh form, 0.5 g (1 + tanh(p / 2)) = g / (1 + e^-p)."""
+    p = g if act == "silu" else math.sqrt(8.0 / math.pi) * (g + 0.044715 * g * g * g)
+    return g / (1.0 + torch.exp(-p))
 
 
 def plain_linear(x, layer, act, dtype):
@@ -241,7 +241,7 @@ def exact(case, seed):
         if case["act"] == "silu":
             return parts[0] * torch.sigmoid(parts[0]) * parts[1]
         if case["act"] == "gelu":
-            return torch.nn.functional.gelu(parts[0], approximate="tanh") * parts[1]
+            return parts[0] * torch.sigmoid((8.0 / math.pi) ** 0.5 * (parts[0] + 0.044715 * parts[0] ** 3)) * parts[1]
         return parts[0]
     x, z = s["x"].double(), s["y"].double()
     if case["post"]:
