@@ -420,7 +420,7 @@ int b200attn_stack_step(b200attn_stack st, int n_rows, b200attn_stream stream);
  *                  normed and rotated q and k, over a sliding window plus the first keep_first positions
  * Feed-forward: down(act(gate x) * up x).
  * ---------------------------------------------------------------------------------------------- */
-typedef enum { B200ATTN_DTYPE_BF16 = 0, B200ATTN_DTYPE_F32 = 1 } b200attn_dtype;
+typedef enum { B200ATTN_DTYPE_BF16 = 0, B200ATTN_DTYPE_F32 = 1, B200ATTN_DTYPE_F16 = 2 /* 8-bit operators only */ } b200attn_dtype;
 typedef enum { B200ATTN_MIXER_MLSTM = 1, B200ATTN_MIXER_LATENT = 2, B200ATTN_MIXER_LIGHTNING = 3, B200ATTN_MIXER_CHANNEL_DELTA = 4,
                B200ATTN_MIXER_DIFF = 5 } b200attn_mixer;
 typedef enum { B200ATTN_ACT_GELU_TANH = 0, B200ATTN_ACT_SILU = 1 } b200attn_act;
@@ -478,6 +478,72 @@ int b200attn_stack_extend(b200attn_stack st, int row, const int* d_tokens, int n
  * stop_after >= 0 makes the following passes end behind that many layer runs, -1 runs all again, -2 changes nothing.
  * No reference counterpart. */
 int b200attn_stack_residual(b200attn_stack st, int rows, float* d_out, int stop_after, b200attn_stream stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Feed-forward in 8-bit integers: the row quantiser, the product with a scale for each token and each output channel, and the norm block.
+ *
+ * A row v is held as int8 codes and one fp32 scale: with a = max |v|, scale = a / 127, code = rint(v * (127 / a)), each operation
+ * rounded once to fp32, ties of the last rounding to even.  A row that holds a NaN or an infinity has the scale NaN and zero codes, so that what is made
+ * of it is NaN; a row whose largest value is below 2^-116 has the scale 0 and zero codes.
+ *
+ * Matrices are row-major with a pitch in elements (>= the columns); element types are b200attn_dtype.  Device pointers need the alignment of their
+ * element type only.  Rows and columns outside a matrix are neither read nor written.  Except where noted, the calls are asynchronous on `stream`,
+ * allocate nothing and may be captured; a call of zero rows does nothing.  Pointers and handles belong to the device that is current.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct b200attn_q8_s* b200attn_q8;   /* weights of an 8-bit product; read-only between calls of set_weights, so that streams may share it */
+
+/* Codes [rows, ld_codes] and scales [rows] of x [rows, cols].  The reference quantises weights this way, in place and by output channel
+ * (src/backend/cuda/kernels/mlp_cuda.cu:22-39); it has no counterpart for activations. */
+int b200attn_q8_quantize(const void* d_x, int dtype, long long ldx, int rows, int cols, int8_t* d_codes, long long ld_codes, float* d_scales,
+                         b200attn_stream stream);
+/* Weights [out, in]; act < 0: one matrix, otherwise (b200attn_act) a gate and an up matrix of that size, whose product is act(gate x) * up x.  in <= 131072:
+ * the sums of a row stay below 2^31.  Allocates.  CudaMLP's weights are quantised at the same granularity (mlp_cuda.cu:22-39). */
+int b200attn_q8_create(int out, int in, int act, b200attn_q8* handle);
+int b200attn_q8_destroy(b200attn_q8 q);      /* No reference counterpart. */
+/* Quantises device matrices of pitch ld per output channel; d_up is null without `act`.  Complete on return.  Reference: mlp_cuda.cu:22-39. */
+int b200attn_q8_set_weights(b200attn_q8 q, const void* d_w, const void* d_up, int dtype, long long ld, b200attn_stream stream);
+/* Copies the weights' codes [out (gated: 2 out, gate first), in] and scales out, for checks.  No reference counterpart. */
+int b200attn_q8_export(b200attn_q8 q, int8_t* d_codes, float* d_scales, b200attn_stream stream);
+/* Bytes of working memory that b200attn_q8_forward wants for so many rows (0: none).  The caller owns it; calls that may overlap need one each.
+ * No reference counterpart. */
+int b200attn_q8_workspace(b200attn_q8 q, int rows, size_t* bytes_out);
+/* y [rows, out] = x W^T from the codes of x and W: (32-bit integer sum) * row scale * channel scale, or act(gate) * up.  accumulate != 0 (plain
+ * fp32 y): added to y.  d_workspace: 16-byte aligned, b200attn_q8_workspace bytes.  x and y must not overlap.  CudaMLP::forward's products
+ * (src/backend/cuda/kernels/mlp_cuda.cu:22-39 for the weights); activations in 8 bits have no counterpart. */
+int b200attn_q8_forward(b200attn_q8 q, const void* d_x, int x_dtype, long long ldx, int rows, void* d_y, int y_dtype, long long ldy, int accumulate,
+                        void* d_workspace, size_t workspace_bytes, b200attn_stream stream);
+/* The same from codes and scales (b200attn_q8_quantize, b200attn_norm_block).  ld_codes a multiple of 16, d_codes 16-byte aligned.
+ * No reference counterpart. */
+int b200attn_q8_forward_codes(b200attn_q8 q, const int8_t* d_codes, long long ld_codes, const float* d_scales, int rows, void* d_y, int y_dtype,
+                              long long ldy, int accumulate, b200attn_stream stream);
+/* Reads (and clears) the device-side status word of the handle's products: 0 = clean, 7 = a bounded wait inside one ran out.  Synchronises the device.
+ * No reference counterpart. */
+int b200attn_q8_device_status(b200attn_q8 q, int* code_out);
+
+typedef enum { B200ATTN_GATE_AS_IS = 0, B200ATTN_GATE_SIGMOID = 1 } b200attn_gate;
+/* The step from one block of a model to the next, for rows of `width` values:
+ *     z = y / sqrt(mean(y^2) + eps) * post_w         (y without d_post_w)
+ *     x' = x_scale * x + y_scale * gate * z          (gate 1 without d_gate; x_scale * x without d_y)
+ *     n = x' / sqrt(mean(x'^2) + eps) * pre_w        (factor 1 without d_pre_w)
+ * in fp32, x' rounded to x_dtype and n to dtype at the end; or n as codes and scales.  width <= 49152. */
+typedef struct {
+    int rows, width;
+    int dtype;                                   /* of y, gate and out                                              */
+    int x_dtype;                                 /* of x and x_out: dtype or B200ATTN_DTYPE_F32                     */
+    const void* d_x; long long ldx;
+    const void* d_y; long long ldy;              /* output of the block, may be null                                */
+    const float* d_post_w;                       /* [width], may be null                                            */
+    const void* d_gate; long long ld_gate;       /* [rows, width], ld_gate 0: one row for all; may be null          */
+    int gate_kind;                               /* b200attn_gate                                                   */
+    float x_scale, y_scale, eps;
+    void* d_x_out; long long ldx_out;            /* x'; d_x with the same pitch (in place) or a buffer of its own; null: not stored */
+    const float* d_pre_w;                        /* [width], may be null                                            */
+    void* d_out; long long ld_out;               /* n, null: not stored                                             */
+    int8_t* d_codes; long long ld_codes;         /* n as codes, null: not stored; d_scales with it                  */
+    float* d_scales;
+} b200attn_norm_args;
+/* No reference counterpart (its norm is src/backend/cuda/kernels/rmsnorm_cuda.cu:90-98). */
+int b200attn_norm_block(const b200attn_norm_args* args, b200attn_stream stream);
 
 /* Number of kernels this library launched on behalf of the calling thread since the last call
  * with reset != 0 (graph replays count the nodes of the captured step).  No reference counterpart. */

@@ -1,7 +1,8 @@
-// Element-type helpers of the kernels that run in bf16 or fp32: conversions, four-element accesses, host dispatch.
+// Element-type helpers of the kernels that run in bf16 or fp32 (some in fp16 too): conversions, four-element accesses, host dispatch.
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -10,9 +11,11 @@ namespace b200 {
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -61,6 +64,12 @@ template <typename F>
 inline void dispatch_elem(ElemType t, F&& f) {
     if (t == ELEM_F32) f(float{});
     else f(__nv_bfloat16{});
+}
+// The same over all three types.
+template <typename F>
+inline void dispatch_elem3(ElemType t, F&& f) {
+    if (t == ELEM_F16) f(__half{});
+    else dispatch_elem(t, f);
 }
 
 }  // namespace b200

@@ -1,0 +1,51 @@
+// 8-bit operators: row quantiser and norm block (q8_rows.cu), products in 8-bit integers (q8_gemm.cu).
+#pragma once
+
+#include "common.cuh"
+
+namespace b200 {
+
+// How a row of values v is held in 8 bits.  With a = max |v|: scale = a / 127, code = rint(v * (127 / a)), every operation rounded once to fp32, so that
+// the codes do not depend on who computes them.  A row with a NaN or an infinity has the scale NaN and zero codes (what is made of it is NaN, not a
+// plausible number); a row below 2^-116 the scale 0 and zero codes (127 / a would overflow).
+struct Q8Row {
+    float scale, inv;
+};
+constexpr uint32_t kQ8Finite = 0x7f800000u;              // bits of |v|: infinities and NaN from here on
+constexpr float kQ8Tiny = 1.2037062152420224e-35f;       // 2^-116
+__device__ __forceinline__ uint32_t q8_abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }      // ordered like |v|, NaN above all
+__device__ __forceinline__ Q8Row q8_row(uint32_t abs_bits) {
+    if (abs_bits >= kQ8Finite) return {__uint_as_float(0x7fc00000u), 0.f};
+    const float a = __uint_as_float(abs_bits);
+    if (a < kQ8Tiny) return {0.f, 0.f};
+    return {__fdiv_rn(a, 127.0f), __fdiv_rn(127.0f, a)};
+}
+// inv = 0: a zero code, also of a NaN or an infinity (the conversion of a NaN is zero).
+__device__ __forceinline__ int q8_code(float v, float inv) { return __float2int_rn(__fmul_rn(v, inv)); }
+
+int launch_q8_quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_t* codes, long long ldc, int pad_to, float* scales, cudaStream_t s);
+constexpr int kNormMostWidth = 49152;                    // an fp32 row in shared memory
+int launch_norm_block(const b200attn_norm_args& a, ElemType x_type, ElemType type, cudaStream_t s);
+
+// Y = (X codes . W codes) * row scale * channel scale, or act(gate) * up of a pair of weights, from X itself (quantised on the way in).
+struct Q8Product {
+    const void* x = nullptr;         // [rows, in]
+    long long ldx = 0;
+    ElemType x_type = ELEM_F16;
+    const int8_t* codes = nullptr;   // or X as codes, pitch a multiple of 16, and scales
+    long long ld_codes = 0;
+    const float* scales = nullptr;
+    int rows = 0, in = 0, out = 0;
+    const int8_t* w = nullptr;       // [out (gated: 2 out, gate rows first), pitch]
+    int pitch = 0;                   // a multiple of 128; columns behind `in` are zeros
+    const float* w_scales = nullptr;
+    int act = -1;                    // b200attn_act of a gated pair, -1: plain
+    void* y = nullptr;
+    long long ldy = 0;
+    ElemType y_type = ELEM_F32;
+    bool accumulate = false;         // fp32 Y: added to what is there
+    int* error = nullptr;
+};
+int q8_few_rows(const Q8Product& p, cudaStream_t s);
+
+}  // namespace b200

@@ -20,9 +20,10 @@ LIB_PATH = os.path.join(_HERE, "libb200attn.so")
 OK, ERR_INVALID, ERR_CUDA, ERR_NOMEM, ERR_NOT_READY, ERR_UNSUPPORTED, ERR_DEVICE = 0, -1, -2, -3, -4, -5, -6
 PROJ_FP32, PROJ_FP16 = 0, 1
 KV_INT8, KV_FP16 = 0, 1
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
 MIXER_MLSTM, MIXER_LATENT, MIXER_LIGHTNING, MIXER_CHANNEL_DELTA, MIXER_DIFF = 1, 2, 3, 4, 5
 ACT_GELU_TANH, ACT_SILU = 0, 1
+GATE_AS_IS, GATE_SIGMOID = 0, 1
 
 # Every symbol include/b200attn.h declares (tests check the library exports exactly these).
 ABI_SYMBOLS = [
@@ -43,6 +44,8 @@ ABI_SYMBOLS = [
     "b200attn_decode_graph_launch", "b200attn_stack_set_tokens", "b200attn_stack_get_tokens",
     "b200attn_stack_begin_batching", "b200attn_stack_admit", "b200attn_stack_retire", "b200attn_stack_rows", "b200attn_stack_step",
     "b200attn_stack_create_layers", "b200attn_stack_set_tensor", "b200attn_stack_open", "b200attn_stack_extend", "b200attn_stack_residual",
+    "b200attn_q8_quantize", "b200attn_q8_create", "b200attn_q8_destroy", "b200attn_q8_set_weights", "b200attn_q8_export", "b200attn_q8_workspace",
+    "b200attn_q8_forward", "b200attn_q8_forward_codes", "b200attn_q8_device_status", "b200attn_norm_block",
 ]
 
 
@@ -66,6 +69,11 @@ def load_library() -> C.CDLL:
             raise ImportError(f"{LIB_PATH} does not export {name}")
     lib.b200attn_last_error.restype = C.c_char_p
     lib.b200attn_launch_count.restype = C.c_longlong
+    i, ll, p = C.c_int, C.c_longlong, C.c_void_p
+    for name, args in (("q8_quantize", [p, i, ll, i, i, p, ll, p, p]), ("q8_set_weights", [p, p, p, i, ll, p]),
+                       ("q8_workspace", [p, i, C.POINTER(C.c_size_t)]), ("q8_forward", [p, p, i, ll, i, p, i, ll, i, p, C.c_size_t, p]),
+                       ("q8_forward_codes", [p, p, ll, p, i, p, i, ll, i, p]), ("norm_block", [p, p])):
+        getattr(lib, "b200attn_" + name).argtypes = args
     return lib
 
 
@@ -155,6 +163,14 @@ class LayerDesc(C.Structure):
                 ("rot_dim", C.c_int), ("window", C.c_int), ("kv_from", C.c_int), ("rot_base", C.c_double), ("scale", C.c_double), ("ff", C.c_int)] + \
                [(n, C.c_int) for n in ("act", "kv_heads", "conv_taps", "a_rank", "g_rank", "keep_first")] + \
                [("diff", C.c_double), ("decay", C.POINTER(C.c_double))]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [("rows", C.c_int), ("width", C.c_int), ("dtype", C.c_int), ("x_dtype", C.c_int), ("d_x", C.c_void_p), ("ldx", C.c_longlong),
+                ("d_y", C.c_void_p), ("ldy", C.c_longlong), ("d_post_w", C.c_void_p), ("d_gate", C.c_void_p), ("ld_gate", C.c_longlong), ("gate_kind", C.c_int),
+                ("x_scale", C.c_float), ("y_scale", C.c_float), ("eps", C.c_float), ("d_x_out", C.c_void_p), ("ldx_out", C.c_longlong),
+                ("d_pre_w", C.c_void_p), ("d_out", C.c_void_p), ("ld_out", C.c_longlong), ("d_codes", C.c_void_p), ("ld_codes", C.c_longlong),
+                ("d_scales", C.c_void_p)]
 
 
 class LayerWeights(C.Structure):
@@ -383,6 +399,181 @@ class LinearAttention:
                 _lib.b200attn_la_destroy(self.h)
         except Exception:
             pass
+
+
+# ---- feed-forward in 8-bit integers ------------------------------------------------------------------------------------
+_Q8_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32, torch.float16: DTYPE_F16}
+
+
+def _invalid(message: str) -> InvalidArgument:
+    return InvalidArgument(ERR_INVALID, message)
+
+
+def _matrix(t: torch.Tensor, name: str, cols: int | None = None, rows: int | None = None) -> int:
+    """Type code of a [rows, cols] matrix on the current device whose columns lie side by side."""
+    code = _Q8_DTYPES.get(t.dtype)
+    if code is None:
+        raise _invalid(f"{name}: element type {t.dtype}")
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise _invalid(f"{name}: not on the current CUDA device")
+    if t.dim() != 2 or (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
+        raise _invalid(f"{name}: shape {tuple(t.shape)}, wanted [{'rows' if rows is None else rows}, {'columns' if cols is None else cols}]")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise _invalid(f"{name}: strides {t.stride()}; the columns of a row lie side by side and rows do not overlap")
+    return code
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+
+
+def _vector(t: torch.Tensor | None, name: str, n: int) -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.float32 or not t.is_cuda or t.device.index != torch.cuda.current_device() or t.dim() != 1 or t.shape[0] != n or \
+            (n > 1 and t.stride(0) != 1):
+        raise _invalid(f"{name}: {n} contiguous fp32 values on the current CUDA device wanted")
+    return t.data_ptr()
+
+
+def _current_stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _new_codes(rows: int, cols: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes with the row pitch that Int8Linear.forward_codes takes (a multiple of 16), and scales."""
+    pitch = (cols + 15) // 16 * 16
+    codes = torch.empty((rows, pitch), dtype=torch.int8, device=device)
+    return (codes if pitch == cols else codes[:, :cols]), torch.empty(rows, dtype=torch.float32, device=device)
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(int8 codes [rows, cols], fp32 scales [rows]) of fp32, fp16 or bf16 rows; x is about codes * scales[:, None]."""
+    code = _matrix(x, "quantize_rows")
+    rows, cols = x.shape
+    codes, scales = _new_codes(rows, cols, x.device)
+    _check(_lib.b200attn_q8_quantize(x.data_ptr(), code, _pitch(x), rows, cols, codes.data_ptr(), _pitch(codes), scales.data_ptr(), _current_stream()))
+    return codes, scales
+
+
+class Int8Linear:
+    """y = x W^T in 8-bit integers: W quantised per output channel when it is given, x per row in every call."""
+
+    def __init__(self, weight: torch.Tensor):
+        self._create([weight], -1)
+
+    def _create(self, weights: list, act: int) -> None:
+        code = _matrix(weights[0], "weight")
+        self.out_features, self.in_features = weights[0].shape
+        for w in weights[1:]:
+            if _matrix(w, "up", self.in_features, self.out_features) != code or _pitch(w) != _pitch(weights[0]):
+                raise _invalid("gate and up: the same element type and row pitch wanted")
+        self.act, self.dtype = act, weights[0].dtype
+        self.h = C.c_void_p()
+        _check(_lib.b200attn_q8_create(C.c_int(self.out_features), C.c_int(self.in_features), C.c_int(act), C.byref(self.h)))
+        _check(_lib.b200attn_q8_set_weights(self.h, weights[0].data_ptr(), weights[1].data_ptr() if act >= 0 else None, code, _pitch(weights[0]),
+                                            _current_stream()))
+
+    def _output(self, rows: int, device, out_dtype, out, accumulate: bool) -> tuple[torch.Tensor, int]:
+        if out is None:
+            if accumulate:
+                raise _invalid("accumulate wants an output to add to")
+            if out_dtype not in _Q8_DTYPES:
+                raise _invalid(f"output type {out_dtype}")
+            out = torch.empty((rows, self.out_features), dtype=out_dtype, device=device)
+        return out, _matrix(out, "out", self.out_features, rows)
+
+    def forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
+        """[rows, in] -> [rows, out] of out_dtype (default: x's), into `out` if given (fp32 and accumulate: added to it)."""
+        code = _matrix(x, "x", self.in_features)
+        rows = x.shape[0]
+        out, out_code = self._output(rows, x.device, out_dtype or x.dtype, out, accumulate)
+        n = C.c_size_t(0)
+        _check(_lib.b200attn_q8_workspace(self.h, rows, C.byref(n)))
+        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device) if n.value else None
+        _check(_lib.b200attn_q8_forward(self.h, x.data_ptr(), code, _pitch(x), rows, out.data_ptr(), out_code, _pitch(out), int(accumulate),
+                                        ws.data_ptr() if ws is not None else None, n.value, _current_stream()))
+        return out
+
+    def forward_codes(self, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+                      accumulate: bool = False) -> torch.Tensor:
+        """The same from what quantize_rows or norm_block returned."""
+        if codes.dtype != torch.int8 or not codes.is_cuda or codes.device.index != torch.cuda.current_device() or codes.dim() != 2 or \
+                codes.shape[1] != self.in_features or codes.stride(1) != 1:
+            raise _invalid(f"codes: int8 [rows, {self.in_features}] on the current CUDA device wanted")
+        rows = codes.shape[0]
+        out, out_code = self._output(rows, codes.device, out_dtype, out, accumulate)
+        pitch = codes.stride(0) if rows > 1 else (self.in_features + 15) // 16 * 16      # of one row nothing is read behind its columns
+        _check(_lib.b200attn_q8_forward_codes(self.h, codes.data_ptr(), pitch, _vector(scales, "scales", rows), rows, out.data_ptr(), out_code, _pitch(out),
+                                              int(accumulate), _current_stream()))
+        return out
+
+    def weight_codes(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """Codes and scales of the weights, a gated pair's gate rows in front of its up rows."""
+        n = self.out_features * (2 if self.act >= 0 else 1)
+        codes = torch.empty((n, self.in_features), dtype=torch.int8, device="cuda")
+        scales = torch.empty(n, dtype=torch.float32, device="cuda")
+        _check(_lib.b200attn_q8_export(self.h, _dev(codes), _dev(scales), _stream()))
+        return codes, scales
+
+    def device_status(self) -> int:
+        code = C.c_int(0)
+        _check(_lib.b200attn_q8_device_status(self.h, C.byref(code)))
+        return code.value
+
+    def __del__(self):
+        try:
+            if getattr(self, "h", None) and self.h.value:
+                _lib.b200attn_q8_destroy(self.h)
+        except Exception:
+            pass
+
+
+class Int8GatedLinear(Int8Linear):
+    """y = act(x G^T) * (x U^T) in 8-bit integers, act SiLU or tanh-GELU: the first half of a gated feed-forward."""
+
+    def __init__(self, gate: torch.Tensor, up: torch.Tensor, act: int = ACT_SILU):
+        if act not in (ACT_GELU_TANH, ACT_SILU):
+            raise _invalid(f"unknown activation {act}")
+        self._create([gate, up], act)
+
+
+def norm_block(x: torch.Tensor, y: torch.Tensor | None = None, pre_w: torch.Tensor | None = None, post_w: torch.Tensor | None = None,
+               gate: torch.Tensor | None = None, sigmoid_gate: bool = False, x_scale: float = 1.0, y_scale: float = 1.0, eps: float = 1e-6,
+               out_dtype: torch.dtype | None = None, in_place: bool = False):
+    """From one block to the next: x' = x_scale x + y_scale gate(norm(y) post_w), n = norm(x') pre_w.
+
+    y is None (no block output yet) or of the activations' type; post_w None leaves its norm out; gate is [rows, width], [width] or None.  Returns
+    (x', n) with n of `out_dtype` (y's type where there is a y), or (x', codes, scales) when out_dtype is None.  in_place: x' is x.
+    """
+    x_code = _matrix(x, "x")
+    rows, width = x.shape
+    dtype = y.dtype if y is not None else out_dtype if out_dtype is not None else x.dtype
+    if dtype not in _Q8_DTYPES or (out_dtype is not None and out_dtype != dtype):
+        raise _invalid(f"norm_block: output type {out_dtype} for activations of {dtype}")
+    a = NormArgs(rows, width, _Q8_DTYPES[dtype], x_code, x.data_ptr(), _pitch(x))
+    if y is not None:
+        _matrix(y, "y", width, rows)
+        a.d_y, a.ldy = y.data_ptr(), _pitch(y)
+    a.d_post_w, a.d_pre_w = _vector(post_w, "post_w", width), _vector(pre_w, "pre_w", width)
+    if gate is not None:
+        g = gate[None] if gate.dim() == 1 else gate
+        if _matrix(g, "gate", width, 1 if gate.dim() == 1 else rows) != a.dtype:
+            raise _invalid("gate: the type of y wanted")
+        a.d_gate, a.ld_gate, a.gate_kind = g.data_ptr(), 0 if gate.dim() == 1 else _pitch(g), GATE_SIGMOID if sigmoid_gate else GATE_AS_IS
+    a.x_scale, a.y_scale, a.eps = x_scale, y_scale, eps
+    x_out = x if in_place else torch.empty((rows, width), dtype=x.dtype, device=x.device)
+    a.d_x_out, a.ldx_out = x_out.data_ptr(), _pitch(x_out)
+    if out_dtype is None:
+        codes, scales = _new_codes(rows, width, x.device)
+        a.d_codes, a.ld_codes, a.d_scales = codes.data_ptr(), _pitch(codes), scales.data_ptr()
+        result = (x_out, codes, scales)
+    else:
+        n = torch.empty((rows, width), dtype=dtype, device=x.device)
+        a.d_out, a.ld_out = n.data_ptr(), _pitch(n)
+        result = (x_out, n)
+    _check(_lib.b200attn_norm_block(C.addressof(a), _current_stream()))
+    return result
 
 
 # ---- hybrid stack + graph-captured decode -------------------------------------------------------------------------
