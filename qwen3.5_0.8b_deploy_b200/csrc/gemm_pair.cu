@@ -9,6 +9,8 @@
 //               rows of the product and the tokens its columns: a thread holds one channel and finds the taps of a token in its own registers.
 //               65536 rows 950 us (projection 878 and convolution 502 before, 3.2 GB between them), 3 x 333 23 (33), 9 x 466 67 (111).
 //
+//   kPairQ8, kPairQ8Glu   products in 8-bit integers, the sums (32-bit integers) times a scale per row and one per column, as they are or gated
+//
 // A cluster of two CTAs owns a 256 x 256 tile (cta_group::2, M = 256): each CTA fetches its 128 rows of both operands and holds 128 rows of the
 // result, so that an operand byte in shared memory serves twice the products that it would in a tile of one CTA.  Two accumulators of 256 columns
 // fill TMEM; sixteen warps (kPairConv: eight, in turns) empty one while the other is being filled.  Persistent: one CTA per SM, tiles in a fixed order.
@@ -29,7 +31,8 @@ constexpr uint32_t kStage = 2 * kOperand;
 constexpr int kEpiWarps = 16;
 constexpr int kThreads = 32 * (kEpiWarps + 2);          // epilogue warps, one for loads, one for TMEM and (CTA 0) the products
 
-enum { kPairGlu = 0, kPairConv, kPairStore16, kPairStore32 };
+enum { kPairGlu = 0, kPairConv, kPairStore16, kPairStore32, kPairQ8, kPairQ8Glu };
+constexpr bool is_q8(int epi) { return epi == kPairQ8 || epi == kPairQ8Glu; }
 constexpr int kConvTokens = 253;                        // of a tile of 256 columns: the first three are the taps of the fourth
 constexpr int kMaxSeqRows = 512;                        // first rows and slots of the sequences kept in shared memory, up to so many sequences
 
@@ -56,6 +59,10 @@ struct PairArgs {
     int up;                        // kPairGlu: W row of the first up column (0: groups of 32 gate and 32 up rows)
     int* error;
     LaConvArgs la;                 // kPairConv
+    const float *x_scales, *w_scales, *up_scales;      // kPairQ8, kPairQ8Glu: of the rows and the columns, the latter readable up to whole tiles
+    void* y;                       // kPairQ8, kPairQ8Glu: results whose base or pitch no tensor map takes are stored by the threads (null: by TMA)
+    long long ldy;
+    int accumulate;
 };
 
 // One unit of work: a tile, or a part of it `width` columns of the product wide.
@@ -142,6 +149,74 @@ __device__ __forceinline__ void plain_part(const PairArgs& p, const CUtensorMap*
         __syncwarp();
         if (lane == 0) {
             tma_store_2d(map_y, out_smem, col + c, row);
+            bulk_commit_group();
+        }
+        __syncwarp();
+    }
+}
+
+// 32 rows of `cols` columns (kPairQ8Glu: of 32 outputs whose gate and up sums lie at acc and acc_up) as values, 64 bytes of a row at a time.  16-bit
+// results go through the fast exponential and division: together they are off by at most 2^-20 of the value where the rounding takes 2^-12.
+template <int EPI, typename Y, int kAct>
+__device__ __forceinline__ void q8_part(const PairArgs& p, const CUtensorMap* map_y, uint32_t acc, uint32_t acc_up, uint32_t out_smem, unsigned char* out, int row,
+                                        int col, int cols, int lane) {
+    constexpr int kCols = 64 / (int)sizeof(Y);
+    using A = std::conditional_t<std::is_same<Y, float>::value, float, __nv_bfloat16>;
+    if (row >= p.rows) return;
+    const float sx = row + lane < p.rows ? p.x_scales[row + lane] : 0.f;
+#pragma unroll 1
+    for (int c = 0; c < cols && col + c < p.cols; c += kCols) {
+        uint32_t v[kCols], u[kCols];
+        if constexpr (kCols == 32) tmem_ld32(acc + c, v); else tmem_ld16(acc + c, v);
+        if constexpr (EPI == kPairQ8Glu) {
+            if constexpr (kCols == 32) tmem_ld32(acc_up + c, u); else tmem_ld16(acc_up + c, u);
+        }
+        tmem_wait_ld();
+        const float4* sw = reinterpret_cast<const float4*>(p.w_scales + col + c);
+        const float4* su = reinterpret_cast<const float4*>(p.up_scales + col + c);
+#pragma unroll
+        for (int j = 0; j < kCols / 4; ++j) {
+            const float4 s4 = __ldg(sw + j), u4 = EPI == kPairQ8Glu ? __ldg(su + j) : s4;
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w}, us[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float f = (float)(int)v[4 * j + e] * sx * s[e];
+                if constexpr (EPI == kPairQ8Glu) f = activated<A, kAct>(f) * ((float)(int)u[4 * j + e] * sx * us[e]);
+                v[4 * j + e] = __float_as_uint(f);
+            }
+        }
+        uint32_t o[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if constexpr (kCols == 32) o[j] = pack2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), Y{});
+            else o[j] = v[j];
+        }
+        if (lane == 0) bulk_wait_group_read0();          // the last rows have left this place
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(out + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        if (p.y) {
+            __syncwarp();
+            constexpr int kAtOnce = 32 / kCols;          // rows
+            const int at = lane % kCols, n = col + c + at;
+            for (int r = lane / kCols; r < min(32, p.rows - row); r += kAtOnce) {
+                const int chunk = at * (int)sizeof(Y) / 16;
+                const Y value = *reinterpret_cast<const Y*>(out + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4) + at * (int)sizeof(Y) % 16);
+                if (n < p.cols) {
+                    Y* dst = static_cast<Y*>(p.y) + (row + r) * p.ldy + n;
+                    if constexpr (std::is_same<Y, float>::value) *dst = p.accumulate ? *dst + value : value;
+                    else *dst = value;
+                }
+            }
+            __syncwarp();
+            continue;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            if (std::is_same<Y, float>::value && p.accumulate) tma_add_2d(map_y, out_smem, col + c, row);
+            else tma_store_2d(map_y, out_smem, col + c, row);
             bulk_commit_group();
         }
         __syncwarp();
@@ -393,6 +468,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
         tma_prefetch_desc(&maps.b);
         tma_prefetch_desc(&maps.out[0]);
     }
+    constexpr int kSlice = is_q8(EPI) ? 128 : 64;           // elements of a slice
     const PairItem first(p, pair);
     tc_fence_before();
     __syncthreads();
@@ -415,7 +491,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
             const int a_row = (EPI == kPairConv ? w.col : w.row * 256) + rank * 128;
             const int b_row = EPI == kPairConv ? w.row * kConvTokens - 3 + rank * 128 : p.up ? w.col / 2 + rank * p.up : w.col + rank * w.width / 2;
             const uint32_t bytes = 2 * (kOperand + w.width * 64);              // of both CTAs
-            for (int k = 0; k < 64 * p.k_steps; k += 64) {
+            for (int k = 0; k < kSlice * p.k_steps; k += kSlice) {
                 if (!mbar_wait_warp<kClusterScope>(empty(s), parity, abort_flag)) { ok = false; break; }
                 const uint32_t dst = base + s * kStage, bar = landed + 8u * s;
                 if (elect_one()) {
@@ -449,7 +525,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
             for (int t = pair; t < p.items && ok; t += pairs, ++i) {
                 const int b = i & 1;
                 if (t != pair) w = PairItem(p, t);
-                const uint32_t idesc = umma_idesc(fmt, 256, w.width, 0, 0);
+                const uint32_t idesc = is_q8(EPI) ? umma_idesc_i8(256, w.width) : umma_idesc(fmt, 256, w.width, 0, 0);
                 if (!mbar_wait_warp<kClusterScope>(acc_empty(b), ((i >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t d = tmem + b * 256;
@@ -459,9 +535,11 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
                     const uint64_t a = a0 + s * (kStage >> 4), wd = w0 + s * (kStage >> 4);
                     const uint32_t done = empty(s);
                     if (elect_one()) {
-                        umma_f16_pair(d, a, wd, idesc, ks > 0);
 #pragma unroll
-                        for (int kk = 1; kk < 4; ++kk) umma_f16_pair(d, a + 2 * kk, wd + 2 * kk, idesc, 1u);
+                        for (int kk = 0; kk < 4; ++kk) {         // 32 bytes of every row
+                            if constexpr (is_q8(EPI)) umma_i8_pair(d, a + 2 * kk, wd + 2 * kk, idesc, ks > 0 || kk > 0);
+                            else umma_f16_pair(d, a + 2 * kk, wd + 2 * kk, idesc, ks > 0 || kk > 0);
+                        }
                         umma_commit_pair(done);
                     }
                     if (++s == kStages) { s = 0; parity ^= 1; }
@@ -516,7 +594,13 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
             } else {
                 if (!mbar_wait_warp<kClusterScope>(acc_full(b), (i >> 1) & 1, abort_flag)) break;
                 tc_fence_after();
-                if constexpr (EPI != kPairGlu) {
+                if constexpr (is_q8(EPI)) {
+                    const int row = w.row * 256 + rank * 128 + 32 * q;
+                    if (64 * part < w.width) {
+                        if constexpr (EPI == kPairQ8) q8_part<EPI, T, kAct>(p, &maps.out[0], acc + 64 * part, 0, out_smem, out, row, w.col + 64 * part, 64, lane);
+                        else q8_part<EPI, T, kAct>(p, &maps.out[0], acc + 32 * part, acc + 32 * part + w.width / 2, out_smem, out, row, w.col / 2 + 32 * part, 32, lane);
+                    }
+                } else if constexpr (EPI != kPairGlu) {
                     if (64 * part < w.width)
                         plain_part<T, EPI>(p, &maps.out[0], acc + 64 * part, out_smem, out, w.row * 256 + rank * 128 + 32 * q, w.col + 64 * part, lane);
                 } else if (64 * part < w.width)
@@ -568,7 +652,7 @@ int launch_pair(const PairMaps& maps, PairArgs p, cudaStream_t s) {
 }
 
 // [rows, cols] row-major, in boxes of so many columns and rows; a swizzle as wide as the box for operands and (64 bytes) results but those of kPairConv
-int map_rows(CUtensorMap* m, ElemType t, const void* p, long long rows, int cols, int box_cols, int box_rows, bool swizzle = true, int pitch = 0) {
+int map_rows(CUtensorMap* m, ElemType t, const void* p, long long rows, int cols, int box_cols, int box_rows, bool swizzle = true, long long pitch = 0) {
     const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, str[1] = {(uint64_t)(pitch ? pitch : cols) * elem_bytes(t)};
     const uint32_t box[2] = {(uint32_t)box_cols, (uint32_t)box_rows};
     return make_tensor_map(m, t == ELEM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : t == ELEM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
@@ -666,6 +750,48 @@ int gemm_pair(cudaStream_t s, const void* x, int ldx, const void* w, void* y, in
     constexpr int kNone = B200ATTN_ACT_SILU;
     if (in_type == ELEM_F16) return launch_pair<kPairStore32, __half, kNone>(m, p, s);
     return out_type == ELEM_F32 ? launch_pair<kPairStore32, __nv_bfloat16, kNone>(m, p, s) : launch_pair<kPairStore16, __nv_bfloat16, kNone>(m, p, s);
+}
+
+template <typename Y>
+static int launch_pair_q8(const PairMaps& m, const PairArgs& p, int act, cudaStream_t s) {
+    if (act < 0) return launch_pair<kPairQ8, Y, B200ATTN_ACT_SILU>(m, p, s);
+    return act == B200ATTN_ACT_SILU ? launch_pair<kPairQ8Glu, Y, B200ATTN_ACT_SILU>(m, p, s) : launch_pair<kPairQ8Glu, Y, B200ATTN_ACT_GELU_TANH>(m, p, s);
+}
+
+int gemm_pair_q8(cudaStream_t s, const Q8Product& q) {
+    auto map_codes = [&](CUtensorMap* m, const int8_t* codes, long long rows, long long pitch, int box_rows) {
+        const uint64_t dims[2] = {(uint64_t)q.in, (uint64_t)rows}, str[1] = {(uint64_t)pitch};
+        const uint32_t box[2] = {128, (uint32_t)box_rows};
+        return make_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, str, box);
+    };
+    const bool glu = q.act >= 0;
+    const long long w_rows = glu ? 2LL * q.out : q.out;
+    PairMaps m{};
+    B2_TRY(map_codes(&m.a, q.codes, q.rows, q.ld_codes, 128));
+    B2_TRY(map_codes(&m.b, q.w, w_rows, q.pitch, 128));
+    B2_TRY(map_codes(&m.b32, q.w, w_rows, q.pitch, 32));
+    PairArgs p{};
+    p.row_tiles = ceil_div(q.rows, 256);
+    p.col_tiles = ceil_div(q.out, glu ? 128 : 256);
+    p.k_steps = ceil_div(q.in, 128);
+    p.rows = q.rows;
+    p.cols = q.out;
+    p.up = glu ? q.out : 0;
+    p.error = q.error;
+    p.x_scales = q.scales;
+    p.w_scales = q.w_scales;
+    p.up_scales = q.w_scales + q.scale_pitch;
+    p.accumulate = q.accumulate;
+    // TMA clips a row of results at the next multiple of 16 bytes, not at its last column (seen with 515 fp32 columns of 516), so the columns have to end at one.
+    // Codes that are read behind the last column meet zeros of W.
+    if (aligned16(q.y) && q.ldy * elem_bytes(q.y_type) % 16 == 0 && q.out * elem_bytes(q.y_type) % 16 == 0) {
+        B2_TRY(map_rows(&m.out[0], q.y_type, q.y, q.rows, q.out, q.y_type == ELEM_F32 ? 16 : 32, 32, true, q.ldy));
+    } else {
+        p.y = q.y;
+        p.ldy = q.ldy;
+    }
+    if (q.y_type == ELEM_F32) return launch_pair_q8<float>(m, p, q.act, s);
+    return q.y_type == ELEM_F16 ? launch_pair_q8<__half>(m, p, q.act, s) : launch_pair_q8<__nv_bfloat16>(m, p, q.act, s);
 }
 
 }  // namespace b200

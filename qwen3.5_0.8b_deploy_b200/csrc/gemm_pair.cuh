@@ -2,6 +2,7 @@
 #pragma once
 
 #include "kernels.cuh"
+#include "q8.cuh"
 
 namespace b200 {
 
@@ -28,5 +29,8 @@ struct LaConvArgs {
 };
 bool gemm_la_conv_takes(const void* x, const void* w, long long rows, int n_seqs);
 int gemm_la_conv(cudaStream_t s, const __half* x, const __half* w, int rows, const LaConvArgs& la, int* error);
+
+// Products in 8-bit integers of rows that are codes already (p.codes).
+int gemm_pair_q8(cudaStream_t s, const Q8Product& p);
 
 }  // namespace b200

@@ -38,7 +38,8 @@ struct Q8Product {
     int rows = 0, in = 0, out = 0;
     const int8_t* w = nullptr;       // [out (gated: 2 out, gate rows first), pitch]
     int pitch = 0;                   // a multiple of 128; columns behind `in` are zeros
-    const float* w_scales = nullptr;
+    const float* w_scales = nullptr; // readable up to a whole tile of 256 (gated: of 128) columns
+    int scale_pitch = 0;             // gated: from the gate's scales to those of up, a multiple of 4
     int act = -1;                    // b200attn_act of a gated pair, -1: plain
     void* y = nullptr;
     long long ldy = 0;
@@ -46,6 +47,7 @@ struct Q8Product {
     bool accumulate = false;         // fp32 Y: added to what is there
     int* error = nullptr;
 };
+bool q8_few_rows_takes(int rows, int in);      // the others: codes first, then gemm_pair_q8
 int q8_few_rows(const Q8Product& p, cudaStream_t s);
 
 }  // namespace b200

@@ -1,4 +1,4 @@
-// Products in 8-bit integers on mma.sync: Y = (X codes . W codes) * row scale * channel scale for blocks of up to 16 rows, which are quantised on the way in.
+// Products in 8-bit integers on mma.sync: Y = (X codes . W codes) * row scale * channel scale for up to 16 rows, which are quantised on the way in.
 // The sums are 32-bit integers, so the order in which warps and lanes take K does not show.
 #include "elem.cuh"
 #include "ptx_utils.cuh"
@@ -29,7 +29,7 @@ q8_few_rows_kernel(const Q8Product p) {
     __shared__ int s_sum[2][kWarps][128];
     __shared__ float s_scale[kRows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = blockIdx.y * kRows, rows = min(kRows, p.rows - row0), pitch = codes_pitch(p.pitch);
+    const int rows = p.rows, pitch = codes_pitch(p.pitch);
     int8_t* sx = reinterpret_cast<int8_t*>(smem);
     pdl_enter();
     {
@@ -38,11 +38,11 @@ q8_few_rows_kernel(const Q8Product p) {
         if (m >= rows) {
             for (int c = lane; c < p.pitch; c += 32) dst[c] = 0;
         } else if (p.codes) {
-            const int8_t* src = p.codes + (row0 + m) * p.ld_codes;
+            const int8_t* src = p.codes + m * p.ld_codes;
             for (int c = lane; c < p.pitch; c += 32) dst[c] = c < p.in ? src[c] : 0;
-            if (lane == 0) s_scale[m] = p.scales[row0 + m];
+            if (lane == 0) s_scale[m] = p.scales[m];
         } else {
-            const X* src = static_cast<const X*>(p.x) + (row0 + m) * p.ldx;
+            const X* src = static_cast<const X*>(p.x) + m * p.ldx;
             uint32_t top = 0;
             for (int c = lane; c < p.in; c += 32) top = max(top, q8_abs_bits(to_f32(src[c])));
 #pragma unroll
@@ -79,11 +79,11 @@ q8_few_rows_kernel(const Q8Product p) {
                 for (int part = 0; part < parts; ++part) {
                     int sum = 0;
                     for (int i = 0; i < kWarps; ++i) sum += s_sum[part][i][threadIdx.x];
-                    v[part] = (float)sum * s_scale[m] * p.w_scales[part * p.out + n];
+                    v[part] = (float)sum * s_scale[m] * p.w_scales[part * p.scale_pitch + n];
                 }
                 if (p.act == B200ATTN_ACT_SILU) v[0] = activated<float, B200ATTN_ACT_SILU>(v[0]) * v[1];
                 if (p.act == B200ATTN_ACT_GELU_TANH) v[0] = activated<float, B200ATTN_ACT_GELU_TANH>(v[0]) * v[1];
-                Y* y = static_cast<Y*>(p.y) + (row0 + m) * p.ldy + n;
+                Y* y = static_cast<Y*>(p.y) + m * p.ldy + n;
                 if constexpr (std::is_same<Y, float>::value) {
                     if (p.accumulate) v[0] += *y;
                 }
@@ -96,9 +96,9 @@ q8_few_rows_kernel(const Q8Product p) {
 
 }  // namespace
 
+bool q8_few_rows_takes(int rows, int in) { return rows <= kRows && in <= kMostK; }
+
 int q8_few_rows(const Q8Product& p, cudaStream_t s) {
-    if (p.rows == 0) return 0;
-    if (p.pitch > kMostK) B2_FAIL(B200ATTN_ERR_UNSUPPORTED, "8-bit product: depth %d above %d", p.in, kMostK);
     int sms = 0, st = 0;
     B2_TRY(device_sm_count(&sms));
     dispatch_elem3(p.x_type, [&](auto xt) {
@@ -109,7 +109,7 @@ int q8_few_rows(const Q8Product& p, cudaStream_t s) {
                 static PerDeviceOnce once;
                 B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRows * (kMostK + 64))));
                 const int tiles = ceil_div(p.out, 8);
-                launch_pdl(q8_few_rows_kernel<X, Y>, dim3(std::min(tiles, sms), ceil_div(p.rows, kRows)), dim3(kThreads), (size_t)kRows * codes_pitch(p.pitch), s, p);
+                launch_pdl(q8_few_rows_kernel<X, Y>, dim3(std::min(tiles, sms)), dim3(kThreads), (size_t)kRows * codes_pitch(p.pitch), s, p);
                 B2_LAUNCH_CHECK();
                 return 0;
             }();

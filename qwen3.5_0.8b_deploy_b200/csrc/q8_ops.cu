@@ -1,5 +1,5 @@
 // Entry points of the 8-bit operators.
-#include "q8.cuh"
+#include "gemm_pair.cuh"
 
 #include <climits>
 #include <new>
@@ -7,10 +7,10 @@
 using namespace b200;
 
 struct b200attn_q8_s {
-    int out = 0, in = 0, act = -1, pitch = 0, device = 0;
+    int out = 0, in = 0, act = -1, pitch = 0, scale_pitch = 0, device = 0;
     bool ready = false;
     int8_t* d_w = nullptr;       // [rows(), pitch], zeros behind column `in`
-    float* d_scales = nullptr;
+    float* d_scales = nullptr;   // [scale_pitch], gated: [2][scale_pitch]
     int* d_error = nullptr;
     int rows() const { return act >= 0 ? 2 * out : out; }
 };
@@ -35,6 +35,19 @@ int check_handle(b200attn_q8 q, const char* what, bool need_weights) {
     B2_CHECK_ARG(dev == q->device, "%s: the handle belongs to device %d, device %d is current", what, q->device, dev);
     if (need_weights && !q->ready) B2_FAIL(B200ATTN_ERR_NOT_READY, "%s: weights not set", what);
     return 0;
+}
+
+// Codes and scales of rows that are quantised in front of the product.
+size_t codes_bytes(b200attn_q8 q, int rows) { return ((size_t)rows * round_up(q->in, 16) + 255) / 256 * 256; }
+size_t workspace_bytes(b200attn_q8 q, int rows) { return q8_few_rows_takes(rows, q->in) ? 0 : codes_bytes(q, rows) + (size_t)rows * 4; }
+
+Q8Product product_of(b200attn_q8 q, int rows, void* d_y, long long ldy, ElemType y_type, int accumulate) {
+    Q8Product p;
+    p.rows = rows; p.in = q->in; p.out = q->out; p.act = q->act;
+    p.w = q->d_w; p.pitch = q->pitch; p.w_scales = q->d_scales; p.scale_pitch = q->scale_pitch;
+    p.y = d_y; p.ldy = ldy; p.y_type = y_type; p.accumulate = accumulate != 0;
+    p.error = q->d_error;
+    return p;
 }
 
 int check_output(b200attn_q8 q, const char* what, int rows, const void* d_y, int y_dtype, long long ldy, int accumulate, ElemType* yt) {
@@ -71,10 +84,11 @@ extern "C" int b200attn_q8_create(int out, int in, int act, b200attn_q8* handle)
     if (!q) B2_FAIL(B200ATTN_ERR_NOMEM, "q8_create: host allocation failed");
     q->out = out; q->in = in; q->act = act < 0 ? -1 : act;
     q->pitch = round_up(in, kPitchStep);
+    q->scale_pitch = round_up(out, 256);                 // products read scales by whole tiles
     auto fill = [&]() -> int {
         B2_CUDA(cudaGetDevice(&q->device));
         B2_CUDA(cudaMalloc(&q->d_w, (size_t)q->rows() * q->pitch));
-        B2_CUDA(cudaMalloc(&q->d_scales, (size_t)q->rows() * 4));
+        B2_CUDA(cudaMalloc(&q->d_scales, (size_t)q->scale_pitch * (q->act >= 0 ? 8 : 4)));
         B2_CUDA(cudaMalloc(&q->d_error, 4));
         B2_CUDA(cudaMemset(q->d_error, 0, 4));
         B2_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
@@ -103,7 +117,7 @@ extern "C" int b200attn_q8_set_weights(b200attn_q8 q, const void* d_w, const voi
     cudaStream_t s = as_stream(stream);
     q->ready = false;
     B2_TRY(launch_q8_quantize(t, d_w, ld, q->out, q->in, q->d_w, q->pitch, q->pitch, q->d_scales, s));
-    if (d_up) B2_TRY(launch_q8_quantize(t, d_up, ld, q->out, q->in, q->d_w + (size_t)q->out * q->pitch, q->pitch, q->pitch, q->d_scales + q->out, s));
+    if (d_up) B2_TRY(launch_q8_quantize(t, d_up, ld, q->out, q->in, q->d_w + (size_t)q->out * q->pitch, q->pitch, q->pitch, q->d_scales + q->scale_pitch, s));
     B2_CUDA(cudaStreamSynchronize(s));
     q->ready = true;
     return 0;
@@ -113,48 +127,53 @@ extern "C" int b200attn_q8_export(b200attn_q8 q, int8_t* d_codes, float* d_scale
     B2_TRY(check_handle(q, "q8_export", true));
     B2_CHECK_ARG(d_codes && d_scales, "q8_export: null argument");
     B2_CUDA(cudaMemcpy2DAsync(d_codes, q->in, q->d_w, q->pitch, q->in, q->rows(), cudaMemcpyDeviceToDevice, as_stream(stream)));
-    B2_CUDA(cudaMemcpyAsync(d_scales, q->d_scales, (size_t)q->rows() * 4, cudaMemcpyDeviceToDevice, as_stream(stream)));
+    B2_CUDA(cudaMemcpy2DAsync(d_scales, (size_t)q->out * 4, q->d_scales, (size_t)q->scale_pitch * 4, (size_t)q->out * 4, q->act >= 0 ? 2 : 1, cudaMemcpyDeviceToDevice,
+                              as_stream(stream)));
     return 0;
 }
 
 extern "C" int b200attn_q8_workspace(b200attn_q8 q, int rows, size_t* bytes_out) {
     B2_CHECK_ARG(q && bytes_out && rows >= 0, "q8_workspace: bad argument");
-    *bytes_out = 0;
+    *bytes_out = workspace_bytes(q, rows);
     return 0;
 }
 
 extern "C" int b200attn_q8_forward(b200attn_q8 q, const void* d_x, int x_dtype, long long ldx, int rows, void* d_y, int y_dtype, long long ldy, int accumulate,
-                                   void* d_workspace, size_t workspace_bytes, b200attn_stream stream) {
-    Q8Product p;
+                                   void* d_workspace, size_t workspace_size, b200attn_stream stream) {
+    ElemType xt, yt;
     B2_TRY(check_handle(q, "q8_forward", true));
-    B2_TRY(check_output(q, "q8_forward", rows, d_y, y_dtype, ldy, accumulate, &p.y_type));
-    B2_CHECK_ARG(elem_of(x_dtype, &p.x_type), "q8_forward: bad input type %d", x_dtype);
+    B2_TRY(check_output(q, "q8_forward", rows, d_y, y_dtype, ldy, accumulate, &yt));
+    B2_CHECK_ARG(elem_of(x_dtype, &xt), "q8_forward: bad input type %d", x_dtype);
     B2_CHECK_ARG(ldx >= q->in, "q8_forward: input pitch %lld below %d columns", ldx, q->in);
     if (rows == 0) return 0;
-    B2_CHECK_ARG(d_x && aligned_to(d_x, elem_bytes(p.x_type)), "q8_forward: input null or not aligned to its elements");
-    p.x = d_x; p.ldx = ldx;
-    p.rows = rows; p.in = q->in; p.out = q->out; p.act = q->act;
-    p.w = q->d_w; p.pitch = q->pitch; p.w_scales = q->d_scales;
-    p.y = d_y; p.ldy = ldy; p.accumulate = accumulate != 0;
-    p.error = q->d_error;
-    return q8_few_rows(p, as_stream(stream));
+    B2_CHECK_ARG(d_x && aligned_to(d_x, elem_bytes(xt)), "q8_forward: input null or not aligned to its elements");
+    Q8Product p = product_of(q, rows, d_y, ldy, yt, accumulate);
+    cudaStream_t s = as_stream(stream);
+    if (q8_few_rows_takes(rows, q->in)) {
+        p.x = d_x; p.ldx = ldx; p.x_type = xt;
+        return q8_few_rows(p, s);
+    }
+    const size_t need = workspace_bytes(q, rows);
+    B2_CHECK_ARG(d_workspace && aligned_to(d_workspace, 16) && workspace_size >= need, "q8_forward: a workspace of %zu bytes on a 16-byte boundary wanted", need);
+    int8_t* codes = static_cast<int8_t*>(d_workspace);
+    float* scales = reinterpret_cast<float*>(codes + codes_bytes(q, rows));
+    p.codes = codes; p.ld_codes = round_up(q->in, 16); p.scales = scales;
+    B2_TRY(launch_q8_quantize(xt, d_x, ldx, rows, q->in, codes, p.ld_codes, q->in, scales, s));
+    return gemm_pair_q8(s, p);
 }
 
 extern "C" int b200attn_q8_forward_codes(b200attn_q8 q, const int8_t* d_codes, long long ld_codes, const float* d_scales, int rows, void* d_y, int y_dtype,
                                          long long ldy, int accumulate, b200attn_stream stream) {
-    Q8Product p;
+    ElemType yt;
     B2_TRY(check_handle(q, "q8_forward_codes", true));
-    B2_TRY(check_output(q, "q8_forward_codes", rows, d_y, y_dtype, ldy, accumulate, &p.y_type));
+    B2_TRY(check_output(q, "q8_forward_codes", rows, d_y, y_dtype, ldy, accumulate, &yt));
     B2_CHECK_ARG(ld_codes >= q->in && ld_codes % 16 == 0, "q8_forward_codes: pitch %lld for %d columns, a multiple of 16 wanted", ld_codes, q->in);
     if (rows == 0) return 0;
     B2_CHECK_ARG(d_codes && d_scales, "q8_forward_codes: null argument");
     B2_CHECK_ARG(aligned_to(d_codes, 16) && aligned_to(d_scales, 4), "q8_forward_codes: codes not aligned to 16 bytes or scales to 4");
+    Q8Product p = product_of(q, rows, d_y, ldy, yt, accumulate);
     p.codes = d_codes; p.ld_codes = ld_codes; p.scales = d_scales;
-    p.rows = rows; p.in = q->in; p.out = q->out; p.act = q->act;
-    p.w = q->d_w; p.pitch = q->pitch; p.w_scales = q->d_scales;
-    p.y = d_y; p.ldy = ldy; p.accumulate = accumulate != 0;
-    p.error = q->d_error;
-    return q8_few_rows(p, as_stream(stream));
+    return q8_few_rows_takes(rows, q->in) ? q8_few_rows(p, as_stream(stream)) : gemm_pair_q8(as_stream(stream), p);
 }
 
 extern "C" int b200attn_q8_device_status(b200attn_q8 q, int* code_out) {

@@ -138,7 +138,7 @@ def glu_bound(g, u, act, dtype):
 
 SIZES = [(1, 64, 8), (1, 1, 1), (2, 17, 3), (1, 1024, 3584), (3, 1000, 2313), (16, 4096, 515), (15, 128, 64), (16, 7, 40), (17, 256, 96), (31, 1024, 129), (33, 130, 1000),
          (64, 2048, 256), (100, 999, 257), (128, 1024, 1024), (129, 72, 33), (255, 512, 640), (257, 384, 2000), (300, 8192, 31), (777, 1003, 511), (1025, 640, 300), (4, 12000, 90),
-         (2000, 100, 1), (513, 33, 7), (7, 6000, 1000)]
+         (2000, 100, 1), (513, 33, 7), (7, 6000, 1000), (40, 20000, 50), (11, 20000, 50), (2, 131072, 9), (18, 131072, 9)]
 
 
 @pytest.mark.parametrize("rows,cols,out", SIZES)
@@ -223,6 +223,17 @@ def test_rows_without_a_value(ops, cuda, rows):
     w[9, 3] = float("nan")
     y = ops.Int8Linear(w).forward(x)
     assert (y[1, 7] == 0) and torch.isnan(y[1, 9]) and torch.isfinite(y[1, [6, 8, 10]]).all()
+
+
+def test_largest_sums(ops, cuda):
+    """127 * 127 * 131072 = 2114060288 is the largest sum there is."""
+    w = torch.ones(9, 131072, device="cuda")
+    for rows in (1, 20):
+        x = torch.ones(rows, 131072, device="cuda")
+        x[0] = -1
+        want = torch.full((rows, 9), 131072.0, dtype=torch.float64, device="cuda")
+        want[0] *= -1
+        judge(ops.Int8Linear(w).forward(x), want, PLAIN * want.abs(), torch.float32)
 
 
 def test_no_rows(ops, cuda):
