@@ -402,58 +402,57 @@ class LinearAttention:
 
 
 # ---- feed-forward in 8-bit integers ------------------------------------------------------------------------------------
+# A call of a few rows takes the GPU 2 to 4 us, so the checks here are kept short: one pass over what a good call has, reasons only for a bad one.
 _Q8_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32, torch.float16: DTYPE_F16}
+_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _invalid(message: str) -> InvalidArgument:
     return InvalidArgument(ERR_INVALID, message)
 
 
-def _matrix(t: torch.Tensor, name: str, cols: int | None = None, rows: int | None = None) -> int:
-    """Type code of a [rows, cols] matrix on the current device whose columns lie side by side."""
-    code = _Q8_DTYPES.get(t.dtype)
-    if code is None:
-        raise _invalid(f"{name}: element type {t.dtype}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
-        raise _invalid(f"{name}: not on the current CUDA device")
-    if t.dim() != 2 or (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
-        raise _invalid(f"{name}: shape {tuple(t.shape)}, wanted [{'rows' if rows is None else rows}, {'columns' if cols is None else cols}]")
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+def _matrix(t: torch.Tensor, name: str, cols: int = -1, rows: int = -1, types: dict = _Q8_DTYPES) -> tuple[int, int]:
+    """(type code, row pitch) of a [rows, cols] matrix on the current device whose columns lie side by side; -1: any number."""
+    code, shape = types.get(t.dtype, -1), t.shape
+    if code >= 0 and len(shape) == 2 and t.is_cuda and t.get_device() == _device() and (cols < 0 or shape[1] == cols) and (rows < 0 or shape[0] == rows):
+        ld, step = t.stride()
+        if shape[0] <= 1:
+            ld = max(ld, shape[1])
+        if (step == 1 or shape[1] <= 1) and ld >= shape[1]:
+            return code, ld
         raise _invalid(f"{name}: strides {t.stride()}; the columns of a row lie side by side and rows do not overlap")
-    return code
-
-
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    if code < 0:
+        raise _invalid(f"{name}: element type {t.dtype}")
+    if not t.is_cuda or t.get_device() != _device():
+        raise _invalid(f"{name}: not on the current CUDA device")
+    raise _invalid(f"{name}: shape {tuple(shape)}, wanted [{rows if rows >= 0 else 'rows'}, {cols if cols >= 0 else 'columns'}]")
 
 
 def _vector(t: torch.Tensor | None, name: str, n: int) -> int:
     if t is None:
         return 0
-    if t.dtype != torch.float32 or not t.is_cuda or t.device.index != torch.cuda.current_device() or t.dim() != 1 or t.shape[0] != n or \
-            (n > 1 and t.stride(0) != 1):
+    if t.dtype != torch.float32 or not t.is_cuda or t.get_device() != _device() or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         raise _invalid(f"{name}: {n} contiguous fp32 values on the current CUDA device wanted")
     return t.data_ptr()
 
 
 def _current_stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
-
-
-def _new_codes(rows: int, cols: int, device) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes with the row pitch that Int8Linear.forward_codes takes (a multiple of 16), and scales."""
-    pitch = (cols + 15) // 16 * 16
-    codes = torch.empty((rows, pitch), dtype=torch.int8, device=device)
-    return (codes if pitch == cols else codes[:, :cols]), torch.empty(rows, dtype=torch.float32, device=device)
+    return _raw_stream(_device())
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(int8 codes [rows, cols], fp32 scales [rows]) of fp32, fp16 or bf16 rows; x is about codes * scales[:, None]."""
-    code = _matrix(x, "quantize_rows")
+    """(int8 codes [rows, cols], fp32 scales [rows]) of fp32, fp16 or bf16 rows; x is about codes * scales[:, None].  The codes' row pitch is a
+    multiple of 16, as Int8Linear.forward_codes takes it."""
+    code, ld = _matrix(x, "quantize_rows")
     rows, cols = x.shape
-    codes, scales = _new_codes(rows, cols, x.device)
-    _check(_lib.b200attn_q8_quantize(x.data_ptr(), code, _pitch(x), rows, cols, codes.data_ptr(), _pitch(codes), scales.data_ptr(), _current_stream()))
-    return codes, scales
+    pitch = (cols + 15) & -16
+    codes = x.new_empty((rows, pitch), dtype=torch.int8)
+    scales = x.new_empty(rows, dtype=torch.float32)
+    status = _lib.b200attn_q8_quantize(x.data_ptr(), code, ld, rows, cols, codes.data_ptr(), pitch, scales.data_ptr(), _current_stream())
+    if status:
+        _check(status)
+    return (codes if pitch == cols else codes[:, :cols]), scales
 
 
 class Int8Linear:
@@ -463,49 +462,51 @@ class Int8Linear:
         self._create([weight], -1)
 
     def _create(self, weights: list, act: int) -> None:
-        code = _matrix(weights[0], "weight")
+        code, ld = _matrix(weights[0], "weight")
         self.out_features, self.in_features = weights[0].shape
         for w in weights[1:]:
-            if _matrix(w, "up", self.in_features, self.out_features) != code or _pitch(w) != _pitch(weights[0]):
+            if _matrix(w, "up", self.in_features, self.out_features) != (code, ld):
                 raise _invalid("gate and up: the same element type and row pitch wanted")
-        self.act, self.dtype = act, weights[0].dtype
+        self.act = act
         self.h = C.c_void_p()
         _check(_lib.b200attn_q8_create(C.c_int(self.out_features), C.c_int(self.in_features), C.c_int(act), C.byref(self.h)))
-        _check(_lib.b200attn_q8_set_weights(self.h, weights[0].data_ptr(), weights[1].data_ptr() if act >= 0 else None, code, _pitch(weights[0]),
-                                            _current_stream()))
+        _check(_lib.b200attn_q8_set_weights(self.h, weights[0].data_ptr(), weights[1].data_ptr() if act >= 0 else None, code, ld, _current_stream()))
 
-    def _output(self, rows: int, device, out_dtype, out, accumulate: bool) -> tuple[torch.Tensor, int]:
+    def _output(self, x: torch.Tensor, out_dtype, out, accumulate: bool) -> tuple[torch.Tensor, int, int]:
         if out is None:
             if accumulate:
                 raise _invalid("accumulate wants an output to add to")
             if out_dtype not in _Q8_DTYPES:
                 raise _invalid(f"output type {out_dtype}")
-            out = torch.empty((rows, self.out_features), dtype=out_dtype, device=device)
-        return out, _matrix(out, "out", self.out_features, rows)
+            return x.new_empty((x.shape[0], self.out_features), dtype=out_dtype), _Q8_DTYPES[out_dtype], self.out_features
+        return (out, *_matrix(out, "out", self.out_features, x.shape[0]))
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
         """[rows, in] -> [rows, out] of out_dtype (default: x's), into `out` if given (fp32 and accumulate: added to it)."""
-        code = _matrix(x, "x", self.in_features)
+        code, ld = _matrix(x, "x", self.in_features)
+        out, out_code, out_ld = self._output(x, out_dtype or x.dtype, out, accumulate)
         rows = x.shape[0]
-        out, out_code = self._output(rows, x.device, out_dtype or x.dtype, out, accumulate)
         n = C.c_size_t(0)
-        _check(_lib.b200attn_q8_workspace(self.h, rows, C.byref(n)))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device) if n.value else None
-        _check(_lib.b200attn_q8_forward(self.h, x.data_ptr(), code, _pitch(x), rows, out.data_ptr(), out_code, _pitch(out), int(accumulate),
-                                        ws.data_ptr() if ws is not None else None, n.value, _current_stream()))
+        status = _lib.b200attn_q8_workspace(self.h, rows, C.byref(n))
+        ws = x.new_empty(n.value, dtype=torch.uint8) if n.value else None
+        status = status or _lib.b200attn_q8_forward(self.h, x.data_ptr(), code, ld, rows, out.data_ptr(), out_code, out_ld, accumulate,
+                                                    ws.data_ptr() if n.value else None, n.value, _current_stream())
+        if status:
+            _check(status)
         return out
 
     def forward_codes(self, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
                       accumulate: bool = False) -> torch.Tensor:
         """The same from what quantize_rows or norm_block returned."""
-        if codes.dtype != torch.int8 or not codes.is_cuda or codes.device.index != torch.cuda.current_device() or codes.dim() != 2 or \
-                codes.shape[1] != self.in_features or codes.stride(1) != 1:
-            raise _invalid(f"codes: int8 [rows, {self.in_features}] on the current CUDA device wanted")
+        _, ld = _matrix(codes, "codes", self.in_features, types={torch.int8: 0})
+        out, out_code, out_ld = self._output(codes, out_dtype, out, accumulate)
         rows = codes.shape[0]
-        out, out_code = self._output(rows, codes.device, out_dtype, out, accumulate)
-        pitch = codes.stride(0) if rows > 1 else (self.in_features + 15) // 16 * 16      # of one row nothing is read behind its columns
-        _check(_lib.b200attn_q8_forward_codes(self.h, codes.data_ptr(), pitch, _vector(scales, "scales", rows), rows, out.data_ptr(), out_code, _pitch(out),
-                                              int(accumulate), _current_stream()))
+        if rows <= 1:
+            ld = (ld + 15) & -16          # of one row nothing is read behind its columns
+        status = _lib.b200attn_q8_forward_codes(self.h, codes.data_ptr(), ld, _vector(scales, "scales", rows), rows, out.data_ptr(), out_code, out_ld,
+                                                accumulate, _current_stream())
+        if status:
+            _check(status)
         return out
 
     def weight_codes(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -546,33 +547,42 @@ def norm_block(x: torch.Tensor, y: torch.Tensor | None = None, pre_w: torch.Tens
     y is None (no block output yet) or of the activations' type; post_w None leaves its norm out; gate is [rows, width], [width] or None.  Returns
     (x', n) with n of `out_dtype` (y's type where there is a y), or (x', codes, scales) when out_dtype is None.  in_place: x' is x.
     """
-    x_code = _matrix(x, "x")
+    x_code, ldx = _matrix(x, "x")
     rows, width = x.shape
-    dtype = y.dtype if y is not None else out_dtype if out_dtype is not None else x.dtype
-    if dtype not in _Q8_DTYPES or (out_dtype is not None and out_dtype != dtype):
+    dtype = y.dtype if y is not None else out_dtype or x.dtype
+    code = _Q8_DTYPES.get(dtype)
+    if code is None or (out_dtype is not None and out_dtype != dtype):
         raise _invalid(f"norm_block: output type {out_dtype} for activations of {dtype}")
-    a = NormArgs(rows, width, _Q8_DTYPES[dtype], x_code, x.data_ptr(), _pitch(x))
+    a = NormArgs(rows, width, code, x_code, x.data_ptr(), ldx)
     if y is not None:
-        _matrix(y, "y", width, rows)
-        a.d_y, a.ldy = y.data_ptr(), _pitch(y)
-    a.d_post_w, a.d_pre_w = _vector(post_w, "post_w", width), _vector(pre_w, "pre_w", width)
+        a.d_y = y.data_ptr()
+        a.ldy = _matrix(y, "y", width, rows)[1]
+    if post_w is not None:
+        a.d_post_w = _vector(post_w, "post_w", width)
+    if pre_w is not None:
+        a.d_pre_w = _vector(pre_w, "pre_w", width)
     if gate is not None:
-        g = gate[None] if gate.dim() == 1 else gate
-        if _matrix(g, "gate", width, 1 if gate.dim() == 1 else rows) != a.dtype:
+        one = gate.dim() == 1
+        gate = gate[None] if one else gate
+        gate_code, ld = _matrix(gate, "gate", width, 1 if one else rows)
+        if gate_code != code:
             raise _invalid("gate: the type of y wanted")
-        a.d_gate, a.ld_gate, a.gate_kind = g.data_ptr(), 0 if gate.dim() == 1 else _pitch(g), GATE_SIGMOID if sigmoid_gate else GATE_AS_IS
+        a.d_gate, a.ld_gate, a.gate_kind = gate.data_ptr(), 0 if one else ld, GATE_SIGMOID if sigmoid_gate else GATE_AS_IS
     a.x_scale, a.y_scale, a.eps = x_scale, y_scale, eps
-    x_out = x if in_place else torch.empty((rows, width), dtype=x.dtype, device=x.device)
-    a.d_x_out, a.ldx_out = x_out.data_ptr(), _pitch(x_out)
+    x_out = x if in_place else x.new_empty((rows, width))
+    a.d_x_out, a.ldx_out = x_out.data_ptr(), ldx if in_place else width
     if out_dtype is None:
-        codes, scales = _new_codes(rows, width, x.device)
-        a.d_codes, a.ld_codes, a.d_scales = codes.data_ptr(), _pitch(codes), scales.data_ptr()
-        result = (x_out, codes, scales)
+        pitch = (width + 15) & -16
+        codes, scales = x.new_empty((rows, pitch), dtype=torch.int8), x.new_empty(rows, dtype=torch.float32)
+        a.d_codes, a.ld_codes, a.d_scales = codes.data_ptr(), pitch, scales.data_ptr()
+        result = (x_out, codes if pitch == width else codes[:, :width], scales)
     else:
-        n = torch.empty((rows, width), dtype=dtype, device=x.device)
-        a.d_out, a.ld_out = n.data_ptr(), _pitch(n)
+        n = x.new_empty((rows, width), dtype=dtype)
+        a.d_out, a.ld_out = n.data_ptr(), width
         result = (x_out, n)
-    _check(_lib.b200attn_norm_block(C.addressof(a), _current_stream()))
+    status = _lib.b200attn_norm_block(C.addressof(a), _current_stream())
+    if status:
+        _check(status)
     return result
 
 
