@@ -504,15 +504,16 @@ int b200attn_q8_destroy(b200attn_q8 q);      /* No reference counterpart. */
 int b200attn_q8_set_weights(b200attn_q8 q, const void* d_w, const void* d_up, int dtype, long long ld, b200attn_stream stream);
 /* Copies the weights' codes [out (gated: 2 out, gate first), in] and scales out, for checks.  No reference counterpart. */
 int b200attn_q8_export(b200attn_q8 q, int8_t* d_codes, float* d_scales, b200attn_stream stream);
-/* Bytes of working memory that b200attn_q8_forward wants for so many rows (0: none).  The caller owns it; calls that may overlap need one each.
+/* Bytes of working memory that b200attn_q8_forward wants for so many rows of x_dtype (0: none).  The caller owns it; calls that may overlap need one each.
  * No reference counterpart. */
-int b200attn_q8_workspace(b200attn_q8 q, int rows, size_t* bytes_out);
+int b200attn_q8_workspace(b200attn_q8 q, int rows, int x_dtype, size_t* bytes_out);
 /* y [rows, out] = x W^T from the codes of x and W: (32-bit integer sum) * row scale * channel scale, or act(gate) * up.  accumulate != 0 (plain
  * fp32 y): added to y.  d_workspace: 16-byte aligned, b200attn_q8_workspace bytes.  x and y must not overlap.  CudaMLP::forward's products
  * (src/backend/cuda/kernels/mlp_cuda.cu:22-39 for the weights); activations in 8 bits have no counterpart. */
 int b200attn_q8_forward(b200attn_q8 q, const void* d_x, int x_dtype, long long ldx, int rows, void* d_y, int y_dtype, long long ldy, int accumulate,
                         void* d_workspace, size_t workspace_bytes, b200attn_stream stream);
-/* The same from codes and scales (b200attn_q8_quantize, b200attn_norm_block).  ld_codes a multiple of 16, d_codes 16-byte aligned.
+/* The same from codes and scales (b200attn_q8_quantize, b200attn_norm_block).  ld_codes a multiple of 16, d_codes 16-byte aligned; a row is read in
+ * whole 16 bytes, and what lies behind its last column there has no influence.
  * No reference counterpart. */
 int b200attn_q8_forward_codes(b200attn_q8 q, const int8_t* d_codes, long long ld_codes, const float* d_scales, int rows, void* d_y, int y_dtype,
                               long long ldy, int accumulate, b200attn_stream stream);

@@ -497,7 +497,11 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
                 if (elect_one()) {
                     if (rank == 0) mbar_arrive_expect_tx(full(s), bytes);          // the neighbour's bytes may come in first: the phase waits for this arrival
                     tma_load_2d_pair(dst, &maps.a, bar, k, a_row);
-                    if (w.width == 256) tma_load_2d_pair(dst + kOperand, &maps.b, bar, k, b_row);
+                    if constexpr (is_q8(EPI)) {                                    // W in blocks of 8 rows x 128 columns
+                        if (w.width == 256) tma_load_4d_pair(dst + kOperand, &maps.b, bar, 0, 0, k / 128, b_row / 8);
+                        else
+                            for (int r = 0; r < w.width / 2; r += 32) tma_load_4d_pair(dst + kOperand + r * 128, &maps.b32, bar, 0, 0, k / 128, (b_row + r) / 8);
+                    } else if (w.width == 256) tma_load_2d_pair(dst + kOperand, &maps.b, bar, k, b_row);
                     else
                         for (int r = 0; r < w.width / 2; r += 32) tma_load_2d_pair(dst + kOperand + r * 128, &maps.b32, bar, k, b_row + r);
                 }
@@ -759,24 +763,25 @@ static int launch_pair_q8(const PairMaps& m, const PairArgs& p, int act, cudaStr
 }
 
 int gemm_pair_q8(cudaStream_t s, const Q8Product& q) {
-    auto map_codes = [&](CUtensorMap* m, const int8_t* codes, long long rows, long long pitch, int box_rows) {
-        const uint64_t dims[2] = {(uint64_t)q.in, (uint64_t)rows}, str[1] = {(uint64_t)pitch};
-        const uint32_t box[2] = {128, (uint32_t)box_rows};
-        return make_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, str, box);
+    auto map_weights = [&](CUtensorMap* m, int box_rows) {
+        const uint64_t dims[4] = {128, 8, (uint64_t)q.pitch / 128, (uint64_t)q.w_rows / 8}, str[3] = {128, kQ8Block, 8 * (uint64_t)q.pitch};
+        const uint32_t box[4] = {128, 8, 1, (uint32_t)box_rows / 8};
+        return make_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, q.w, dims, str, box);
     };
     const bool glu = q.act >= 0;
-    const long long w_rows = glu ? 2LL * q.out : q.out;
     PairMaps m{};
-    B2_TRY(map_codes(&m.a, q.codes, q.rows, q.ld_codes, 128));
-    B2_TRY(map_codes(&m.b, q.w, w_rows, q.pitch, 128));
-    B2_TRY(map_codes(&m.b32, q.w, w_rows, q.pitch, 32));
+    const uint64_t dims[2] = {(uint64_t)q.in, (uint64_t)q.rows}, str[1] = {(uint64_t)q.ld_codes};
+    const uint32_t box[2] = {128, 128};
+    B2_TRY(make_tensor_map(&m.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q.codes, dims, str, box));
+    B2_TRY(map_weights(&m.b, 128));
+    B2_TRY(map_weights(&m.b32, 32));
     PairArgs p{};
     p.row_tiles = ceil_div(q.rows, 256);
     p.col_tiles = ceil_div(q.out, glu ? 128 : 256);
     p.k_steps = ceil_div(q.in, 128);
     p.rows = q.rows;
     p.cols = q.out;
-    p.up = glu ? q.out : 0;
+    p.up = glu ? q.up_row : 0;
     p.error = q.error;
     p.x_scales = q.scales;
     p.w_scales = q.w_scales;

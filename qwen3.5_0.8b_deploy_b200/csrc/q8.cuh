@@ -22,8 +22,25 @@ __device__ __forceinline__ Q8Row q8_row(uint32_t abs_bits) {
 }
 // inv = 0: a zero code, also of a NaN or an infinity (the conversion of a NaN is zero).
 __device__ __forceinline__ int q8_code(float v, float inv) { return __float2int_rn(__fmul_rn(v, inv)); }
+// Four codes in the bytes of a word.  1.5 * 2^23 added to a product of at most 127.00001 leaves its nearest integer, ties to even, in the low byte: the same as
+// a conversion, at the rate of additions.
+__device__ __forceinline__ uint32_t q8_codes4(float a, float b, float c, float d, float inv) {
+    auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f)); };
+    const uint32_t ab = __byte_perm(code(a), code(b), 0x0040), cd = __byte_perm(code(c), code(d), 0x0040);
+    return inv == 0.f ? 0u : __byte_perm(ab, cd, 0x5410);
+}
 
-int launch_q8_quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_t* codes, long long ldc, int pad_to, float* scales, cudaStream_t s);
+// Codes of rows lie one behind the other (pitch ldc); those of weights in blocks of 8 rows x 128 columns, a block's rows of 128 bytes side by side and
+// the blocks of eight rows one behind the other: what eight output columns want of K is one stretch of memory, and a block is the unit in which shared memory
+// is swizzled for the tensor cores.
+constexpr int kQ8Block = 8 * 128;
+__host__ __device__ __forceinline__ size_t q8_block_offset(long long row, int col, int pitch) {
+    return (size_t)(row / 8) * 8 * pitch + (size_t)(col / 128) * kQ8Block + row % 8 * 128 + col % 128;
+}
+int launch_q8_quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_t* codes, long long ldc, float* scales, cudaStream_t s);
+// pitch: columns rounded up to a multiple of 128, with zeros behind `cols`.
+int launch_q8_quantize_weights(ElemType t, const void* w, long long ldw, int rows, int cols, int8_t* codes, int pitch, float* scales, cudaStream_t s);
+int launch_q8_unblock(const int8_t* codes, int pitch, int rows, int cols, int8_t* out, cudaStream_t s);      // to rows of `cols`
 constexpr int kNormMostWidth = 49152;                    // an fp32 row in shared memory
 int launch_norm_block(const b200attn_norm_args& a, ElemType x_type, ElemType type, cudaStream_t s);
 
@@ -36,7 +53,8 @@ struct Q8Product {
     long long ld_codes = 0;
     const float* scales = nullptr;
     int rows = 0, in = 0, out = 0;
-    const int8_t* w = nullptr;       // [out (gated: 2 out, gate rows first), pitch]
+    const int8_t* w = nullptr;       // in blocks (q8_block_offset); gated: up's rows from `up_row` on, a multiple of 8
+    int up_row = 0, w_rows = 0;      // w_rows: of all, a multiple of 8
     int pitch = 0;                   // a multiple of 128; columns behind `in` are zeros
     const float* w_scales = nullptr; // readable up to a whole tile of 256 (gated: of 128) columns
     int scale_pitch = 0;             // gated: from the gate's scales to those of up, a multiple of 4
@@ -47,7 +65,8 @@ struct Q8Product {
     bool accumulate = false;         // fp32 Y: added to what is there
     int* error = nullptr;
 };
-bool q8_few_rows_takes(int rows, int in);      // the others: codes first, then gemm_pair_q8
+bool q8_few_rows_takes(int rows, int in);      // the others: gemm_pair_q8, from codes
+bool q8_few_rows_quantizes(int rows, int in, ElemType x_type);       // of those: X need not be codes
 int q8_few_rows(const Q8Product& p, cudaStream_t s);
 
 }  // namespace b200

@@ -9,10 +9,11 @@ using namespace b200;
 struct b200attn_q8_s {
     int out = 0, in = 0, act = -1, pitch = 0, scale_pitch = 0, device = 0;
     bool ready = false;
-    int8_t* d_w = nullptr;       // [rows(), pitch], zeros behind column `in`
+    int8_t* d_w = nullptr;       // in blocks (q8_block_offset), zeros behind column `in`; gated: up's rows from up_row() on
     float* d_scales = nullptr;   // [scale_pitch], gated: [2][scale_pitch]
     int* d_error = nullptr;
-    int rows() const { return act >= 0 ? 2 * out : out; }
+    int up_row() const { return (out + 7) / 8 * 8; }
+    int rows() const { return act >= 0 ? 2 * up_row() : up_row(); }
 };
 
 namespace {
@@ -39,12 +40,15 @@ int check_handle(b200attn_q8 q, const char* what, bool need_weights) {
 
 // Codes and scales of rows that are quantised in front of the product.
 size_t codes_bytes(b200attn_q8 q, int rows) { return ((size_t)rows * round_up(q->in, 16) + 255) / 256 * 256; }
-size_t workspace_bytes(b200attn_q8 q, int rows) { return q8_few_rows_takes(rows, q->in) ? 0 : codes_bytes(q, rows) + (size_t)rows * 4; }
+size_t workspace_bytes(b200attn_q8 q, int rows, ElemType xt) {
+    return rows == 0 || (q8_few_rows_takes(rows, q->in) && q8_few_rows_quantizes(rows, q->in, xt)) ? 0 : codes_bytes(q, rows) + (size_t)rows * 4;
+}
+int product(const Q8Product& p, cudaStream_t s) { return q8_few_rows_takes(p.rows, p.in) ? q8_few_rows(p, s) : gemm_pair_q8(s, p); }
 
 Q8Product product_of(b200attn_q8 q, int rows, void* d_y, long long ldy, ElemType y_type, int accumulate) {
     Q8Product p;
     p.rows = rows; p.in = q->in; p.out = q->out; p.act = q->act;
-    p.w = q->d_w; p.pitch = q->pitch; p.w_scales = q->d_scales; p.scale_pitch = q->scale_pitch;
+    p.w = q->d_w; p.up_row = q->up_row(); p.w_rows = q->rows(); p.pitch = q->pitch; p.w_scales = q->d_scales; p.scale_pitch = q->scale_pitch;
     p.y = d_y; p.ldy = ldy; p.y_type = y_type; p.accumulate = accumulate != 0;
     p.error = q->d_error;
     return p;
@@ -71,7 +75,7 @@ extern "C" int b200attn_q8_quantize(const void* d_x, int dtype, long long ldx, i
     if (rows == 0) return 0;
     B2_CHECK_ARG(d_x && d_codes && d_scales, "q8_quantize: null argument");
     B2_CHECK_ARG(aligned_to(d_x, elem_bytes(t)) && aligned_to(d_scales, 4), "q8_quantize: pointer not aligned to its elements");
-    return launch_q8_quantize(t, d_x, ldx, rows, cols, d_codes, ld_codes, cols, d_scales, as_stream(stream));
+    return launch_q8_quantize(t, d_x, ldx, rows, cols, d_codes, ld_codes, d_scales, as_stream(stream));
 }
 
 extern "C" int b200attn_q8_create(int out, int in, int act, b200attn_q8* handle) {
@@ -116,8 +120,9 @@ extern "C" int b200attn_q8_set_weights(b200attn_q8 q, const void* d_w, const voi
     B2_CHECK_ARG(aligned_to(d_w, elem_bytes(t)) && aligned_to(d_up, elem_bytes(t)), "q8_set_weights: pointer not aligned to its elements");
     cudaStream_t s = as_stream(stream);
     q->ready = false;
-    B2_TRY(launch_q8_quantize(t, d_w, ld, q->out, q->in, q->d_w, q->pitch, q->pitch, q->d_scales, s));
-    if (d_up) B2_TRY(launch_q8_quantize(t, d_up, ld, q->out, q->in, q->d_w + (size_t)q->out * q->pitch, q->pitch, q->pitch, q->d_scales + q->scale_pitch, s));
+    B2_TRY(launch_q8_quantize_weights(t, d_w, ld, q->out, q->in, q->d_w, q->pitch, q->d_scales, s));
+    if (d_up)
+        B2_TRY(launch_q8_quantize_weights(t, d_up, ld, q->out, q->in, q->d_w + (size_t)q->up_row() * q->pitch, q->pitch, q->d_scales + q->scale_pitch, s));
     B2_CUDA(cudaStreamSynchronize(s));
     q->ready = true;
     return 0;
@@ -126,15 +131,19 @@ extern "C" int b200attn_q8_set_weights(b200attn_q8 q, const void* d_w, const voi
 extern "C" int b200attn_q8_export(b200attn_q8 q, int8_t* d_codes, float* d_scales, b200attn_stream stream) {
     B2_TRY(check_handle(q, "q8_export", true));
     B2_CHECK_ARG(d_codes && d_scales, "q8_export: null argument");
-    B2_CUDA(cudaMemcpy2DAsync(d_codes, q->in, q->d_w, q->pitch, q->in, q->rows(), cudaMemcpyDeviceToDevice, as_stream(stream)));
+    B2_TRY(launch_q8_unblock(q->d_w, q->pitch, q->out, q->in, d_codes, as_stream(stream)));
+    if (q->act >= 0)
+        B2_TRY(launch_q8_unblock(q->d_w + (size_t)q->up_row() * q->pitch, q->pitch, q->out, q->in, d_codes + (size_t)q->out * q->in, as_stream(stream)));
     B2_CUDA(cudaMemcpy2DAsync(d_scales, (size_t)q->out * 4, q->d_scales, (size_t)q->scale_pitch * 4, (size_t)q->out * 4, q->act >= 0 ? 2 : 1, cudaMemcpyDeviceToDevice,
                               as_stream(stream)));
     return 0;
 }
 
-extern "C" int b200attn_q8_workspace(b200attn_q8 q, int rows, size_t* bytes_out) {
+extern "C" int b200attn_q8_workspace(b200attn_q8 q, int rows, int x_dtype, size_t* bytes_out) {
+    ElemType xt;
     B2_CHECK_ARG(q && bytes_out && rows >= 0, "q8_workspace: bad argument");
-    *bytes_out = workspace_bytes(q, rows);
+    B2_CHECK_ARG(elem_of(x_dtype, &xt), "q8_workspace: bad input type %d", x_dtype);
+    *bytes_out = workspace_bytes(q, rows, xt);
     return 0;
 }
 
@@ -149,17 +158,17 @@ extern "C" int b200attn_q8_forward(b200attn_q8 q, const void* d_x, int x_dtype, 
     B2_CHECK_ARG(d_x && aligned_to(d_x, elem_bytes(xt)), "q8_forward: input null or not aligned to its elements");
     Q8Product p = product_of(q, rows, d_y, ldy, yt, accumulate);
     cudaStream_t s = as_stream(stream);
-    if (q8_few_rows_takes(rows, q->in)) {
+    const size_t need = workspace_bytes(q, rows, xt);
+    if (need == 0) {
         p.x = d_x; p.ldx = ldx; p.x_type = xt;
         return q8_few_rows(p, s);
     }
-    const size_t need = workspace_bytes(q, rows);
     B2_CHECK_ARG(d_workspace && aligned_to(d_workspace, 16) && workspace_size >= need, "q8_forward: a workspace of %zu bytes on a 16-byte boundary wanted", need);
     int8_t* codes = static_cast<int8_t*>(d_workspace);
     float* scales = reinterpret_cast<float*>(codes + codes_bytes(q, rows));
     p.codes = codes; p.ld_codes = round_up(q->in, 16); p.scales = scales;
-    B2_TRY(launch_q8_quantize(xt, d_x, ldx, rows, q->in, codes, p.ld_codes, q->in, scales, s));
-    return gemm_pair_q8(s, p);
+    B2_TRY(launch_q8_quantize(xt, d_x, ldx, rows, q->in, codes, p.ld_codes, scales, s));
+    return product(p, s);
 }
 
 extern "C" int b200attn_q8_forward_codes(b200attn_q8 q, const int8_t* d_codes, long long ld_codes, const float* d_scales, int rows, void* d_y, int y_dtype,
@@ -173,7 +182,7 @@ extern "C" int b200attn_q8_forward_codes(b200attn_q8 q, const int8_t* d_codes, l
     B2_CHECK_ARG(aligned_to(d_codes, 16) && aligned_to(d_scales, 4), "q8_forward_codes: codes not aligned to 16 bytes or scales to 4");
     Q8Product p = product_of(q, rows, d_y, ldy, yt, accumulate);
     p.codes = d_codes; p.ld_codes = ld_codes; p.scales = d_scales;
-    return q8_few_rows_takes(rows, q->in) ? q8_few_rows(p, as_stream(stream)) : gemm_pair_q8(as_stream(stream), p);
+    return product(p, as_stream(stream));
 }
 
 extern "C" int b200attn_q8_device_status(b200attn_q8 q, int* code_out) {

@@ -43,6 +43,14 @@ __device__ __forceinline__ void load_once(const T* p, Raw<T, 8>& r) {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.v[0]), "=r"(r.v[1]), "=r"(r.v[2]), "=r"(r.v[3]) : "l"(p));
 }
 
+// Where a row's code of a column lies, from its first one on.
+template <bool kBlocks>
+__device__ __forceinline__ int code_place(int col) { return kBlocks ? col / 128 * kQ8Block + col % 128 : col; }
+template <bool kBlocks>
+__device__ __forceinline__ int8_t* code_row(int8_t* codes, long long row, long long pitch) {
+    return codes + (kBlocks ? row / 8 * 8 * pitch + row % 8 * 128 : row * pitch);
+}
+
 template <int kRun>
 struct Eight {
     int first, threads, cols;
@@ -104,26 +112,20 @@ struct Eight {
                 if (has(j)) row[col(j)] = from_f32<T>(v[j]);
         }
     }
+    template <bool kBlocks = false>
     __device__ __forceinline__ void store_codes(int8_t* row, const float (&v)[8], const Q8Row& q) const {
-        const uint32_t lo = codes4(v[0], v[1], v[2], v[3], q), hi = codes4(v[4], v[5], v[6], v[7], q);
+        const uint32_t lo = q8_codes4(v[0], v[1], v[2], v[3], q.inv), hi = q8_codes4(v[4], v[5], v[6], v[7], q.inv);
         if constexpr (kRun == 8) {
-            *reinterpret_cast<uint2*>(row + first) = make_uint2(lo, hi);
+            *reinterpret_cast<uint2*>(row + code_place<kBlocks>(first)) = make_uint2(lo, hi);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j += kRun) {
                 if (!has(j)) continue;
                 const uint32_t c = (j < 4 ? lo : hi) >> (8 * (j & 3));
-                if constexpr (kRun == 2) *reinterpret_cast<uint16_t*>(row + col(j)) = (uint16_t)c;
-                else row[col(j)] = (int8_t)c;
+                if constexpr (kRun == 2) *reinterpret_cast<uint16_t*>(row + code_place<kBlocks>(col(j))) = (uint16_t)c;
+                else row[code_place<kBlocks>(col(j))] = (int8_t)c;
             }
         }
-    }
-    // 1.5 * 2^23 added to a product of at most 127.00001 leaves its nearest integer, ties to even, in the low byte: the same as a conversion, at the rate of
-    // additions.  Rows that are held as zeros may have NaN products.
-    __device__ __forceinline__ static uint32_t codes4(float a, float b, float c, float d, const Q8Row& q) {
-        auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, q.inv), 12582912.0f)); };
-        const uint32_t ab = __byte_perm(code(a), code(b), 0x0040), cd = __byte_perm(code(c), code(d), 0x0040);
-        return q.inv == 0.f ? 0u : __byte_perm(ab, cd, 0x5410);
     }
 };
 
@@ -150,16 +152,16 @@ __device__ __forceinline__ V row_reduce(V v, V* part, F f) {
 // ---- quantiser ------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int kBlockThreads = 512;               // most threads of a row
 constexpr int kQuantGroups = 4;                  // eights of a thread
-template <typename T, bool kWarp, int kRun>
+template <typename T, bool kWarp, int kRun, bool kBlocks>
 __global__ void __launch_bounds__(kWarp ? 128 : kBlockThreads)
-q8_quantize_kernel(const T* __restrict__ x, long long ldx, int rows, int cols, int8_t* __restrict__ codes, long long ldc, int pad_to, float* __restrict__ scales) {
+q8_quantize_kernel(const T* __restrict__ x, long long ldx, int rows, int cols, int8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
     __shared__ uint32_t s_max[32];
     const int threads = kWarp ? 32 : blockDim.x, t = kWarp ? threadIdx.x & 31 : threadIdx.x;
     const long long row = kWarp ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     pdl_enter();
     if (row >= rows) return;
     const T* src = x + row * ldx;
-    int8_t* out = codes + row * ldc;
+    int8_t* out = code_row<kBlocks>(codes, row, ldc);
     Raw<T, kRun> raw[kQuantGroups];
 #pragma unroll
     for (int i = 0; i < kQuantGroups; ++i) Eight<kRun>(i, t, threads, cols).template fetch<true>(src, raw[i]);
@@ -177,27 +179,35 @@ q8_quantize_kernel(const T* __restrict__ x, long long ldx, int rows, int cols, i
         const Eight<kRun> e(i, t, threads, cols);
         if (!e.any()) break;
         Eight<kRun>::unpack(raw[i], v);
-        e.store_codes(out, v, q);
+        e.template store_codes<kBlocks>(out, v, q);
     }
-    for (int c = cols + t; c < pad_to; c += threads) out[c] = 0;
+    if constexpr (kBlocks)
+        for (int c = cols + t; c < ldc; c += threads) out[code_place<true>(c)] = 0;
     if (t == 0) scales[row] = q.scale;
 }
 
 // A block per row, two passes over it.
 constexpr int kLoopThreads = kBlockThreads;
-template <typename T>
+template <typename T, bool kBlocks>
 __global__ void __launch_bounds__(kLoopThreads)
-q8_quantize_loop_kernel(const T* __restrict__ x, long long ldx, int cols, int8_t* __restrict__ codes, long long ldc, int pad_to, float* __restrict__ scales) {
+q8_quantize_loop_kernel(const T* __restrict__ x, long long ldx, int cols, int8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
     __shared__ uint32_t s_max[32];
     pdl_enter();
     const T* row = x + blockIdx.x * ldx;
-    int8_t* out = codes + blockIdx.x * ldc;
+    int8_t* out = code_row<kBlocks>(codes, blockIdx.x, ldc);
     uint32_t m = 0;
     for (int c = threadIdx.x; c < cols; c += kLoopThreads) m = max(m, q8_abs_bits(to_f32(row[c])));
     const Q8Row q = q8_row(row_reduce<false>(m, s_max, RowMax{}));
-    for (int c = threadIdx.x; c < cols; c += kLoopThreads) out[c] = (int8_t)q8_code(to_f32(row[c]), q.inv);
-    for (int c = cols + threadIdx.x; c < pad_to; c += kLoopThreads) out[c] = 0;
+    for (int c = threadIdx.x; c < cols; c += kLoopThreads) out[code_place<kBlocks>(c)] = (int8_t)q8_code(to_f32(row[c]), q.inv);
+    if constexpr (kBlocks)
+        for (int c = cols + threadIdx.x; c < ldc; c += kLoopThreads) out[code_place<true>(c)] = 0;
     if (threadIdx.x == 0) scales[blockIdx.x] = q.scale;
+}
+
+__global__ void __launch_bounds__(256)
+q8_unblock_kernel(const int8_t* __restrict__ codes, int pitch, int cols, int8_t* __restrict__ out) {
+    pdl_enter();
+    for (int c = threadIdx.x; c < cols; c += 256) out[(size_t)blockIdx.x * cols + c] = codes[q8_block_offset(blockIdx.x, c, pitch)];
 }
 
 // ---- norm block -----------------------------------------------------------------------------------------------------------------------------------------
@@ -375,12 +385,24 @@ void dispatch_run(int run, F&& f) {
 }
 int threads_for(int cols, int groups) { return std::max(64, (ceil_div(cols, 8 * groups) + 31) / 32 * 32); }
 
-template <typename T, int kRun>
-void quantize(const T* x, long long ldx, int rows, int cols, int8_t* codes, long long ldc, int pad_to, float* scales, cudaStream_t s) {
-    if (cols <= 32 * 8 * kQuantGroups)
-        launch_pdl(q8_quantize_kernel<T, true, kRun>, dim3(ceil_div(rows, 4)), dim3(128), 0, s, x, ldx, rows, cols, codes, ldc, pad_to, scales);
-    else
-        launch_pdl(q8_quantize_kernel<T, false, kRun>, dim3(rows), dim3(threads_for(cols, kQuantGroups)), 0, s, x, ldx, rows, cols, codes, ldc, pad_to, scales);
+template <bool kBlocks>
+int quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_t* codes, long long ldc, float* scales, cudaStream_t s) {
+    if (rows == 0) return 0;
+    dispatch_elem3(t, [&](auto tag) {
+        using T = decltype(tag);
+        const T* src = static_cast<const T*>(x);
+        dispatch_run(std::min(run_of(cols, x, ldx, sizeof(T)), run_of(cols, codes, ldc, 1)), [&](auto run) {
+            constexpr int kRun = decltype(run)::value;
+            if (cols <= 32 * 8 * kQuantGroups)
+                launch_pdl(q8_quantize_kernel<T, true, kRun, kBlocks>, dim3(ceil_div(rows, 4)), dim3(128), 0, s, src, ldx, rows, cols, codes, ldc, scales);
+            else if (cols <= kBlockThreads * 8 * kQuantGroups)
+                launch_pdl(q8_quantize_kernel<T, false, kRun, kBlocks>, dim3(rows), dim3(threads_for(cols, kQuantGroups)), 0, s, src, ldx, rows, cols, codes, ldc, scales);
+            else
+                launch_pdl(q8_quantize_loop_kernel<T, kBlocks>, dim3(rows), dim3(kLoopThreads), 0, s, src, ldx, cols, codes, ldc, scales);
+        });
+    });
+    B2_LAUNCH_CHECK();
+    return 0;
 }
 
 template <typename X, typename T, int kRun>
@@ -401,17 +423,15 @@ int norm_block(const b200attn_norm_args& a, cudaStream_t s) {
 
 }  // namespace
 
-int launch_q8_quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_t* codes, long long ldc, int pad_to, float* scales, cudaStream_t s) {
-    if (rows == 0) return 0;
-    dispatch_elem3(t, [&](auto tag) {
-        using T = decltype(tag);
-        const T* src = static_cast<const T*>(x);
-        if (cols > kBlockThreads * 8 * kQuantGroups)
-            launch_pdl(q8_quantize_loop_kernel<T>, dim3(rows), dim3(kLoopThreads), 0, s, src, ldx, cols, codes, ldc, pad_to, scales);
-        else
-            dispatch_run(std::min(run_of(cols, x, ldx, sizeof(T)), run_of(cols, codes, ldc, 1)),
-                         [&](auto run) { quantize<T, decltype(run)::value>(src, ldx, rows, cols, codes, ldc, pad_to, scales, s); });
-    });
+int launch_q8_quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_t* codes, long long ldc, float* scales, cudaStream_t s) {
+    return quantize<false>(t, x, ldx, rows, cols, codes, ldc, scales, s);
+}
+int launch_q8_quantize_weights(ElemType t, const void* w, long long ldw, int rows, int cols, int8_t* codes, int pitch, float* scales, cudaStream_t s) {
+    return quantize<true>(t, w, ldw, rows, cols, codes, pitch, scales, s);
+}
+
+int launch_q8_unblock(const int8_t* codes, int pitch, int rows, int cols, int8_t* out, cudaStream_t s) {
+    launch_pdl(q8_unblock_kernel, dim3(rows), dim3(256), 0, s, codes, pitch, cols, out);
     B2_LAUNCH_CHECK();
     return 0;
 }

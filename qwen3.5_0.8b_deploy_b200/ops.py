@@ -71,7 +71,7 @@ def load_library() -> C.CDLL:
     lib.b200attn_launch_count.restype = C.c_longlong
     i, ll, p = C.c_int, C.c_longlong, C.c_void_p
     for name, args in (("q8_quantize", [p, i, ll, i, i, p, ll, p, p]), ("q8_set_weights", [p, p, p, i, ll, p]),
-                       ("q8_workspace", [p, i, C.POINTER(C.c_size_t)]), ("q8_forward", [p, p, i, ll, i, p, i, ll, i, p, C.c_size_t, p]),
+                       ("q8_workspace", [p, i, i, C.POINTER(C.c_size_t)]), ("q8_forward", [p, p, i, ll, i, p, i, ll, i, p, C.c_size_t, p]),
                        ("q8_forward_codes", [p, p, ll, p, i, p, i, ll, i, p]), ("norm_block", [p, p])):
         getattr(lib, "b200attn_" + name).argtypes = args
     return lib
@@ -487,7 +487,7 @@ class Int8Linear:
         out, out_code, out_ld = self._output(x, out_dtype or x.dtype, out, accumulate)
         rows = x.shape[0]
         n = C.c_size_t(0)
-        status = _lib.b200attn_q8_workspace(self.h, rows, C.byref(n))
+        status = _lib.b200attn_q8_workspace(self.h, rows, code, C.byref(n))
         ws = x.new_empty(n.value, dtype=torch.uint8) if n.value else None
         status = status or _lib.b200attn_q8_forward(self.h, x.data_ptr(), code, ld, rows, out.data_ptr(), out_code, out_ld, accumulate,
                                                     ws.data_ptr() if n.value else None, n.value, _current_stream())
@@ -502,7 +502,7 @@ class Int8Linear:
         out, out_code, out_ld = self._output(codes, out_dtype, out, accumulate)
         rows = codes.shape[0]
         if rows <= 1:
-            ld = (ld + 15) & -16          # of one row nothing is read behind its columns
+            ld = (ld + 15) & -16          # one row, which may come without the pitch of a matrix
         status = _lib.b200attn_q8_forward_codes(self.h, codes.data_ptr(), ld, _vector(scales, "scales", rows), rows, out.data_ptr(), out_code, out_ld,
                                                 accumulate, _current_stream())
         if status:

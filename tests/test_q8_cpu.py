@@ -32,7 +32,7 @@ def test_product_refusals(ops):
     assert lib.b200attn_q8_create(C.c_int(8), C.c_int(131073), C.c_int(-1), C.byref(h)) == ops.ERR_UNSUPPORTED
     refused(ops, lib.b200attn_q8_create(C.c_int(8), C.c_int(8), C.c_int(-1), None), b"null")
     n = C.c_size_t()
-    refused(ops, lib.b200attn_q8_workspace(None, 4, C.byref(n)), b"q8_workspace")
+    refused(ops, lib.b200attn_q8_workspace(None, 4, 0, C.byref(n)), b"q8_workspace")
     refused(ops, lib.b200attn_q8_forward(None, 4096, 0, 64, 2, 4096, 0, 64, 0, None, 0, None), b"null handle")
     refused(ops, lib.b200attn_q8_forward_codes(None, 4096, 64, 4096, 2, 4096, 0, 64, 0, None), b"null handle")
     refused(ops, lib.b200attn_q8_set_weights(None, 4096, None, 0, 64, None), b"null handle")
