@@ -38,10 +38,10 @@ constexpr int kMaxSeqRows = 512;                        // first rows and slots 
 
 template <int EPI>
 struct PairSmem {
-    static constexpr int kStages = EPI == kPairConv ? 5 : 6;               // ring of 64-deep slices, 32 KB each per CTA
+    static constexpr int kStages = EPI == kPairConv || is_q8(EPI) ? 5 : 6; // ring of 128-byte slices, 32 KB each per CTA
     static constexpr uint32_t kOut = kStages * kStage;                     // 2 KB per epilogue warp
-    static constexpr uint32_t kExtra = kOut + kEpiWarps * 2048;            // kPairConv: the tables of conv_part
-    static constexpr uint32_t kBars = kExtra + (EPI == kPairConv ? 4096 + 4096 + 2048 + 8 * kMaxSeqRows : 0);
+    static constexpr uint32_t kExtra = kOut + kEpiWarps * 2048;            // kPairConv: the tables of conv_part, 8-bit products: 64 scales per epilogue warp
+    static constexpr uint32_t kBars = kExtra + (EPI == kPairConv ? 4096 + 4096 + 2048 + 8 * kMaxSeqRows : is_q8(EPI) ? kEpiWarps * 256 : 0);
     static constexpr int kReaders = EPI == kPairConv ? kEpiWarps / 2 : kEpiWarps;     // epilogue warps of one tile
     static constexpr uint32_t kBytes = kBars + 256 + 1024;
 };
@@ -50,6 +50,7 @@ struct PairMaps {
     CUtensorMap out[4];            // results: kPairGlu one, kPairConv q, k, v, mixed
 };
 
+enum { kStoreRows = 0, kStoreTma, kStoreWords };         // how 8-bit products store their results: see q8_store
 struct PairArgs {
     int row_tiles, col_tiles;      // tiles of X rows and of W rows
     int whole, split_log2;         // of the tiles in their order, `whole` are done as such, each one behind them in 1 << split_log2 narrower parts
@@ -60,9 +61,9 @@ struct PairArgs {
     int* error;
     LaConvArgs la;                 // kPairConv
     const float *x_scales, *w_scales, *up_scales;      // kPairQ8, kPairQ8Glu: of the rows and the columns, the latter readable up to whole tiles
-    void* y;                       // kPairQ8, kPairQ8Glu: results whose base or pitch no tensor map takes are stored by the threads (null: by TMA)
+    void* y;                       // of kPairQ8, kPairQ8Glu
     long long ldy;
-    int accumulate;
+    int store, accumulate;         // kStoreRows ..; results are added to fp32 y
 };
 
 // One unit of work: a tile, or a part of it `width` columns of the product wide.
@@ -155,71 +156,122 @@ __device__ __forceinline__ void plain_part(const PairArgs& p, const CUtensorMap*
     }
 }
 
-// 32 rows of `cols` columns (kPairQ8Glu: of 32 outputs whose gate and up sums lie at acc and acc_up) as values, 64 bytes of a row at a time.  16-bit
-// results go through the fast exponential and division: together they are off by at most 2^-20 of the value where the rounding takes 2^-12.
-template <int EPI, typename Y, int kAct>
-__device__ __forceinline__ void q8_part(const PairArgs& p, const CUtensorMap* map_y, uint32_t acc, uint32_t acc_up, uint32_t out_smem, unsigned char* out, int row,
-                                        int col, int cols, int lane) {
+// ---- kPairQ8, kPairQ8Glu: a warp has 32 rows (one a lane) of 64 columns, or of 32 outputs with their gate and up sums -------------------------------
+// What a lane brings of an item's scales: its row's, and those of two columns (plain: 32 apart, gated: of gate and up).  They are asked for an item ahead and
+// handed round through shared memory, so that nothing in the epilogue waits for memory.
+struct Q8Scales {
+    float row = 0.f, first = 0.f, second = 0.f;
+};
+template <int EPI>
+__device__ __forceinline__ Q8Scales q8_scales(const PairArgs& p, int row, int col, int lane) {
+    Q8Scales s;
+    if (row + lane < p.rows) s.row = __ldg(p.x_scales + row + lane);
+    if (col < p.cols) {
+        s.first = __ldg(p.w_scales + col + lane);
+        s.second = __ldg((EPI == kPairQ8Glu ? p.up_scales + col : p.w_scales + col + 32) + lane);
+    }
+    return s;
+}
+
+// 64 bytes of results of this lane's row, from column col on.  16-bit rows on 32-byte boundaries are stored as they are: 32 lines to a store, but few stores.  The
+// others turn around in shared memory (2 KB of the warp).  From there TMA takes them, or the lanes where y has no tensor map: a word each, 16-bit rows shifted to
+// where such a store may go.  fp32 results of 8192 x 1024 -> 32768 (1.07 GB): 295 us by TMA, 313 in rows of 128 bytes (which cost a slice of the ring), 294 in
+// stores of 16 bytes a lane (the shared memory, which the products read too, was busy for 83 % of the time), 321 straight from the registers.
+template <typename Y>
+__device__ __forceinline__ void q8_store(const PairArgs& p, const CUtensorMap* map_y, const uint32_t (&o)[16], uint32_t stage_smem, unsigned char* stage, int row,
+                                         int col, int lane) {
     constexpr int kCols = 64 / (int)sizeof(Y);
-    using A = std::conditional_t<std::is_same<Y, float>::value, float, __nv_bfloat16>;
-    if (row >= p.rows) return;
-    const float sx = row + lane < p.rows ? p.x_scales[row + lane] : 0.f;
-#pragma unroll 1
-    for (int c = 0; c < cols && col + c < p.cols; c += kCols) {
-        uint32_t v[kCols], u[kCols];
-        if constexpr (kCols == 32) tmem_ld32(acc + c, v); else tmem_ld16(acc + c, v);
-        if constexpr (EPI == kPairQ8Glu) {
-            if constexpr (kCols == 32) tmem_ld32(acc_up + c, u); else tmem_ld16(acc_up + c, u);
-        }
-        tmem_wait_ld();
-        const float4* sw = reinterpret_cast<const float4*>(p.w_scales + col + c);
-        const float4* su = reinterpret_cast<const float4*>(p.up_scales + col + c);
+    const int rows = min(32, p.rows - row), cols = min(kCols, p.cols - col);
+    Y* const first = static_cast<Y*>(p.y) + row * p.ldy + col;
+    if constexpr (sizeof(Y) == 2) {
+        if (p.store == kStoreRows && cols == kCols) {
+            if (lane >= rows) return;
+            Y* dst = first + lane * p.ldy;
 #pragma unroll
-        for (int j = 0; j < kCols / 4; ++j) {
-            const float4 s4 = __ldg(sw + j), u4 = EPI == kPairQ8Glu ? __ldg(su + j) : s4;
-            const float s[4] = {s4.x, s4.y, s4.z, s4.w}, us[4] = {u4.x, u4.y, u4.z, u4.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float f = (float)(int)v[4 * j + e] * sx * s[e];
-                if constexpr (EPI == kPairQ8Glu) f = activated<A, kAct>(f) * ((float)(int)u[4 * j + e] * sx * us[e]);
-                v[4 * j + e] = __float_as_uint(f);
-            }
+            for (int j = 0; j < 16; j += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + j * 2), "r"(o[j]), "r"(o[j + 1]), "r"(o[j + 2]), "r"(o[j + 3]), "r"(o[j + 4]),
+                             "r"(o[j + 5]), "r"(o[j + 6]), "r"(o[j + 7]) : "memory");
+            return;
         }
-        uint32_t o[16];
+    }
+    auto chunk = [&](int r, int c) { return stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };      // as the tensor map swizzles
+    if (p.store == kStoreTma && lane == 0) bulk_wait_group_read0();          // the last rows have left this place
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            if constexpr (kCols == 32) o[j] = pack2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), Y{});
-            else o[j] = v[j];
-        }
-        if (lane == 0) bulk_wait_group_read0();          // the last rows have left this place
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(out + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-        if (p.y) {
-            __syncwarp();
-            constexpr int kAtOnce = 32 / kCols;          // rows
-            const int at = lane % kCols, n = col + c + at;
-            for (int r = lane / kCols; r < min(32, p.rows - row); r += kAtOnce) {
-                const int chunk = at * (int)sizeof(Y) / 16;
-                const Y value = *reinterpret_cast<const Y*>(out + r * 64 + ((chunk ^ ((r >> 1) & 3)) << 4) + at * (int)sizeof(Y) % 16);
-                if (n < p.cols) {
-                    Y* dst = static_cast<Y*>(p.y) + (row + r) * p.ldy + n;
-                    if constexpr (std::is_same<Y, float>::value) *dst = p.accumulate ? *dst + value : value;
-                    else *dst = value;
-                }
-            }
-            __syncwarp();
-            continue;
-        }
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(chunk(lane, j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+    if (p.store == kStoreTma) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-            if (std::is_same<Y, float>::value && p.accumulate) tma_add_2d(map_y, out_smem, col + c, row);
-            else tma_store_2d(map_y, out_smem, col + c, row);
+            if (sizeof(Y) == 4 && p.accumulate) tma_add_2d(map_y, stage_smem, col, row);
+            else tma_store_2d(map_y, stage_smem, col, row);
             bulk_commit_group();
         }
-        __syncwarp();
+        return;
+    }
+    __syncwarp();
+    const int h = lane >> 4, w = lane & 15;                  // rows h, h + 2, ...; word w of each
+    Y* dst = first + h * p.ldy + w * (4 / (int)sizeof(Y));
+    const bool odd = sizeof(Y) == 2 && reinterpret_cast<uintptr_t>(dst) & 2;         // columns 2 w + 1 and 2 w + 2 share a word of y, in every one of these rows
+    const int c = sizeof(Y) == 2 ? 2 * w + odd : w;
+    const bool pair = c + 1 < cols, single = c < cols;
+#pragma unroll 4
+    for (int i = 0; i < 32; i += 2, dst += 2 * p.ldy) {
+        if (i >= rows) break;
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(chunk(i + h, w >> 2) + (w & 3) * 4);
+        const bool live = i + h < rows;
+        if constexpr (sizeof(Y) == 4) {
+            if (live && single) *dst = p.accumulate ? *dst + __uint_as_float(word) : __uint_as_float(word);
+        } else {
+            const uint32_t next = __shfl_down_sync(0xffffffffu, word, 1, 16), both = odd ? __funnelshift_r(word, next, 16) : word;
+            uint16_t* out = reinterpret_cast<uint16_t*>(dst);
+            if (!live) continue;
+            if (odd && w == 0) out[0] = (uint16_t)word;
+            if (pair) *reinterpret_cast<uint32_t*>(out + odd) = both;
+            else if (single) out[odd] = (uint16_t)both;
+        }
+    }
+}
+
+// first: sums of the columns from col on (gated: of the gate), second: of those 32 further on (gated: of up).  16-bit results go through the fast exponential and
+// division: together they are off by at most 2^-20 of the value where the rounding takes 2^-12.
+template <int EPI, typename Y, int kAct, typename Release>
+__device__ __forceinline__ void q8_part(const PairArgs& p, const CUtensorMap* map_y, uint32_t first, uint32_t second, const float* scales, uint32_t stage_smem,
+                                        unsigned char* stage, int row, int col, float sx, int lane, Release&& release) {
+    constexpr int kCols = 64 / (int)sizeof(Y), kAll = EPI == kPairQ8Glu ? 32 : 64;
+    using A = std::conditional_t<std::is_same<Y, float>::value, float, __nv_bfloat16>;
+    uint32_t a[32], b[32];
+    tmem_ld32(first, a);
+    tmem_ld32(second, b);
+    tmem_wait_ld();
+    release();                                   // everything is in registers: the next products may have this place
+    auto value = [&](uint32_t sum, float s) { return (float)(int)sum * sx * s; };
+#pragma unroll
+    for (int c = 0; c < kAll; c += kCols) {
+        if (col + c >= p.cols) break;
+        uint32_t o[16];
+#pragma unroll
+        for (int j = 0; j < kCols; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(scales + c + j);
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = value((c + j + e < 32 ? a : b)[(c + j + e) & 31], s[e]);
+            if constexpr (EPI == kPairQ8Glu) {
+                const float4 u4 = *reinterpret_cast<const float4*>(scales + 32 + c + j);
+                const float u[4] = {u4.x, u4.y, u4.z, u4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = activated<A, kAct>(v[e]) * value(b[c + j + e], u[e]);
+            }
+            if constexpr (sizeof(Y) == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j + e] = __float_as_uint(v[e]);
+            } else {
+                o[j / 2] = pack2(v[0], v[1], Y{});
+                o[j / 2 + 1] = pack2(v[2], v[3], Y{});
+            }
+        }
+        q8_store<Y>(p, map_y, o, stage_smem, stage, row, col + c, lane);
     }
 }
 
@@ -466,7 +518,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
     if (warp == kEpiWarps && lane == 0) {
         tma_prefetch_desc(&maps.a);
         tma_prefetch_desc(&maps.b);
-        tma_prefetch_desc(&maps.out[0]);
+        if constexpr (!is_q8(EPI)) tma_prefetch_desc(&maps.out[0]);
     }
     constexpr int kSlice = is_q8(EPI) ? 128 : 64;           // elements of a slice
     const PairItem first(p, pair);
@@ -564,6 +616,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
         // and stores; all on one tile went through them in step.
         int i = EPI == kPairConv ? warp >> 3 : 0;
         bool ok = true;
+        Q8Scales ahead;
         if constexpr (EPI == kPairConv) {
             int* first_rows = reinterpret_cast<int*>(sm + Smem::kExtra + 10240);
             for (int j = threadIdx.x; j < min(p.la.n_seqs, kMaxSeqRows); j += 32 * kEpiWarps) {
@@ -596,14 +649,34 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
                 tc_fence_after();
                 conv_part(p.la, maps, ok, acc, w.col >> 8, t_tile, p.rows, rank, q, side, lane, info, first_rows, sums, 4 + 2 * half + side, scale, out, release);
             } else {
+                auto q8_row = [&](const PairItem& it) { return it.row * 256 + rank * 128 + 32 * q; };
+                auto q8_col = [&](const PairItem& it) { return 64 * part < it.width ? (EPI == kPairQ8 ? it.col + 64 * part : it.col / 2 + 32 * part) : p.cols; };
+                const bool q8_mine = is_q8(EPI) && q8_row(w) < p.rows && q8_col(w) < p.cols;
+                float sx = 0.f, *scales = reinterpret_cast<float*>(sm + Smem::kExtra + warp * 256);
+                if constexpr (is_q8(EPI)) {
+                    if (t == pair) ahead = q8_scales<EPI>(p, q8_row(w), q8_col(w), lane);
+                    sx = ahead.row;
+                    scales[lane] = ahead.first;
+                    scales[32 + lane] = ahead.second;
+                    __syncwarp();
+                    if (t + pairs < p.items) {
+                        const PairItem next(p, t + pairs);
+                        ahead = q8_scales<EPI>(p, q8_row(next), q8_col(next), lane);
+                    }
+                }
                 if (!mbar_wait_warp<kClusterScope>(acc_full(b), (i >> 1) & 1, abort_flag)) break;
                 tc_fence_after();
                 if constexpr (is_q8(EPI)) {
-                    const int row = w.row * 256 + rank * 128 + 32 * q;
-                    if (64 * part < w.width) {
-                        if constexpr (EPI == kPairQ8) q8_part<EPI, T, kAct>(p, &maps.out[0], acc + 64 * part, 0, out_smem, out, row, w.col + 64 * part, 64, lane);
-                        else q8_part<EPI, T, kAct>(p, &maps.out[0], acc + 32 * part, acc + 32 * part + w.width / 2, out_smem, out, row, w.col / 2 + 32 * part, 32, lane);
-                    }
+                    const uint32_t first_col = acc + (EPI == kPairQ8 ? 64 : 32) * part, second_col = first_col + (EPI == kPairQ8 ? 32 : w.width / 2);
+                    auto early = [&] {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(cluster_smem_addr(acc_empty(b), 0));
+                    };
+                    if (q8_mine) q8_part<EPI, T, kAct>(p, &maps.out[0], first_col, second_col, scales, out_smem, out, q8_row(w), q8_col(w), sx, lane, early);
+                    else early();
+                    __syncwarp();
+                    continue;
                 } else if constexpr (EPI != kPairGlu) {
                     if (64 * part < w.width)
                         plain_part<T, EPI>(p, &maps.out[0], acc + 64 * part, out_smem, out, w.row * 256 + rank * 128 + 32 * q, w.col + 64 * part, lane);
@@ -786,15 +859,14 @@ int gemm_pair_q8(cudaStream_t s, const Q8Product& q) {
     p.x_scales = q.scales;
     p.w_scales = q.w_scales;
     p.up_scales = q.w_scales + q.scale_pitch;
-    p.accumulate = q.accumulate;
+    p.y = q.y;
+    p.ldy = q.ldy;
     // TMA clips a row of results at the next multiple of 16 bytes, not at its last column (seen with 515 fp32 columns of 516), so the columns have to end at one.
     // Codes that are read behind the last column meet zeros of W.
-    if (aligned16(q.y) && q.ldy * elem_bytes(q.y_type) % 16 == 0 && q.out * elem_bytes(q.y_type) % 16 == 0) {
-        B2_TRY(map_rows(&m.out[0], q.y_type, q.y, q.rows, q.out, q.y_type == ELEM_F32 ? 16 : 32, 32, true, q.ldy));
-    } else {
-        p.y = q.y;
-        p.ldy = q.ldy;
-    }
+    const size_t e = elem_bytes(q.y_type), row = (size_t)q.ldy * e;
+    p.store = e == 2 && reinterpret_cast<uintptr_t>(q.y) % 32 == 0 && row % 32 == 0 ? kStoreRows : aligned16(q.y) && row % 16 == 0 && q.out * e % 16 == 0 ? kStoreTma : kStoreWords;
+    if (p.store == kStoreTma) B2_TRY(map_rows(&m.out[0], q.y_type, q.y, q.rows, q.out, e == 4 ? 16 : 32, 32, true, q.ldy));
+    p.accumulate = q.accumulate;
     if (q.y_type == ELEM_F32) return launch_pair_q8<float>(m, p, q.act, s);
     return q.y_type == ELEM_F16 ? launch_pair_q8<__half>(m, p, q.act, s) : launch_pair_q8<__nv_bfloat16>(m, p, q.act, s);
 }

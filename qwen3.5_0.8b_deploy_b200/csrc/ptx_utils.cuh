@@ -113,6 +113,10 @@ __device__ __forceinline__ uint32_t cluster_smem_addr(uint32_t local_smem_addr, 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same without the wait for this thread's earlier stores, where nothing that was written is handed over.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 
 // Every thread of every CTA of the cluster (threads that have exited do not count).
 __device__ __forceinline__ void cluster_sync_all() {
