@@ -314,7 +314,9 @@ typedef struct {
     int kv_dtype;          /* b200attn_kv_dtype */
     int int8_weights;      /* 1: every matrix is quantised per output channel to INT8 codes (scale = absmax/127,
                               roundf; src/backend/cuda/kernels/mlp_cuda.cu:22-39) and the GEMMs use code*scale,
-                              stored as fp16: the values are the INT8 ones, the bytes streamed are fp16 */
+                              stored as fp16: the values are the INT8 ones, the bytes streamed are fp16.
+                              2: the same, but the feed-forward's matrices stay codes and its products run in 8-bit
+                              integers, activations quantised per token (b200attn_q8_*, b200attn_norm_block) */
     float rms_eps;         /* 1e-6 */
 } b200attn_stack_config;
 

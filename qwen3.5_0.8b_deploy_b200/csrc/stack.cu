@@ -241,6 +241,16 @@ static int upload_matrix(const float* h, int rows, int cols, bool int8, __half**
     return st;
 }
 
+// Host fp32 matrices [rows, cols] into an 8-bit product.
+static int set_q8_weights(b200attn_q8 q, const float* h_w, const float* h_up, int rows, int cols) {
+    float *w = nullptr, *up = nullptr;
+    int st = upload_f32(h_w, &w, (size_t)rows * cols);
+    if (st == 0 && h_up) st = upload_f32(h_up, &up, (size_t)rows * cols);
+    if (st == 0) st = b200attn_q8_set_weights(q, w, up, B200ATTN_DTYPE_F32, cols, nullptr);
+    cudaFree(w); cudaFree(up);
+    return st;
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -255,6 +265,9 @@ extern "C" int b200attn_stack_destroy(b200attn_stack st) {
     for (auto p : st->d_post_norm) cudaFree(p);
     for (auto p : st->d_wgu) cudaFree(p);
     for (auto p : st->d_wdown) cudaFree(p);
+    for (auto q : st->q8_gu) b200attn_q8_destroy(q);
+    for (auto q : st->q8_down) b200attn_q8_destroy(q);
+    cudaFree(st->d_codes); cudaFree(st->d_code_scales); cudaFree(st->d_q8_work);
     cudaFree(st->d_embed); cudaFree(st->d_final_norm);
     b200attn_kv_pool_destroy(st->pool);
     b200attn_la_state_destroy(st->state);
@@ -284,6 +297,7 @@ extern "C" int b200attn_stack_create(const b200attn_stack_config* cfg, b200attn_
     }
     st->d_in_norm.assign(L, nullptr); st->d_post_norm.assign(L, nullptr);
     st->d_wgu.assign(L, nullptr); st->d_wdown.assign(L, nullptr);
+    st->q8_gu.assign(L, nullptr); st->q8_down.assign(L, nullptr);
     st->layer_ready.assign(L, 0);
     st->max_rows = std::max(cfg->max_seqs, cfg->prefill_chunk_seqs * cfg->max_seq_len);
     int rc = 0;
@@ -338,6 +352,17 @@ extern "C" int b200attn_stack_create(const b200attn_stack_config* cfg, b200attn_
     ST_CUDA(cudaMalloc(&st->d_error, sizeof(int)));
     ST_CUDA(cudaMemset(st->d_error, 0, sizeof(int)));
     ST_CUDA(cudaMalloc(&st->d_last_idx, (size_t)cfg->max_seqs * 4));
+    if (st->q8_ffn()) {
+        for (int i = 0; i < L; ++i) {
+            if ((rc = b200attn_q8_create(cfg->intermediate_size, kHidden, B200ATTN_ACT_SILU, &st->q8_gu[i])) != 0) return fail(rc);
+            if ((rc = b200attn_q8_create(kHidden, cfg->intermediate_size, -1, &st->q8_down[i])) != 0) return fail(rc);
+        }
+        // the most that a pass may want: of the rows it may have, passes of few rows may want none
+        if ((rc = b200attn_q8_workspace(st->q8_down[0], std::max(st->max_rows, kRowsGemmMax + 1), B200ATTN_DTYPE_F16, &st->q8_work_bytes)) != 0) return fail(rc);
+        ST_CUDA(cudaMalloc(&st->d_codes, R * kHidden));
+        ST_CUDA(cudaMalloc(&st->d_code_scales, R * 4));
+        ST_CUDA(cudaMalloc(&st->d_q8_work, st->q8_work_bytes));
+    }
     iota_kernel<<<ceil_div(cfg->max_seqs, 128), 128>>>(st->d_slots, cfg->max_seqs);
     ST_CUDA(cudaDeviceSynchronize());
 #undef ST_CUDA
@@ -359,9 +384,13 @@ extern "C" int b200attn_stack_set_layer_weights(b200attn_stack st, int layer, co
     // rows (after quantisation, so the INT8 codes are those of the original matrix): x / rms * (1 + w) W^T = x / rms W'^T.
     // The norm kernels of the unfused paths therefore run with zero weights, and the fused decode step needs no norm
     // launch at all: its projections scale their output rows by 1 / rms.
+    // A feed-forward in 8-bit integers takes the norm's factors themselves: its matrices stay codes.
     const std::vector<float> zeros(kHidden, 0.f);
     B2_TRY(upload_f32(zeros.data(), &st->d_in_norm[layer], kHidden));
-    B2_TRY(upload_f32(zeros.data(), &st->d_post_norm[layer], kHidden));
+    std::vector<float> post(kHidden, 0.f);
+    if (st->q8_ffn())
+        for (int c = 0; c < kHidden; ++c) post[c] = 1.0f + w->post_norm[c];
+    B2_TRY(upload_f32(post.data(), &st->d_post_norm[layer], kHidden));
     // Per-output-channel INT8 fake quantisation on the host (the arithmetic of quantize_rows_kernel).
     auto q8_copy = [&](const float* src, int rows, int cols, std::vector<float>& dst) {
         dst.assign(src, src + (size_t)rows * cols);
@@ -381,7 +410,10 @@ extern "C" int b200attn_stack_set_layer_weights(b200attn_stack st, int layer, co
             for (int c = 0; c < kHidden; ++c) row[c] *= 1.0f + norm_w[c];
         }
     };
-    {
+    if (st->q8_ffn()) {
+        B2_TRY(set_q8_weights(st->q8_gu[layer], w->ffn_gate, w->ffn_up, inter, kHidden));
+        B2_TRY(set_q8_weights(st->q8_down[layer], w->ffn_down, nullptr, kHidden, inter));
+    } else {
         // rows in tiles of 64: 32 gate rows then the 32 matching up rows (see swiglu_kernel)
         std::vector<float> gu_src((size_t)2 * inter * kHidden), gu;
         for (int c = 0; c < inter; ++c) {
@@ -392,8 +424,8 @@ extern "C" int b200attn_stack_set_layer_weights(b200attn_stack st, int layer, co
         q8_copy(gu_src.data(), 2 * inter, kHidden, gu);
         fold(gu, 2 * inter, w->post_norm);
         B2_TRY(upload_matrix(gu.data(), 2 * inter, kHidden, false, &st->d_wgu[layer]));
+        B2_TRY(upload_matrix(w->ffn_down, kHidden, inter, q8, &st->d_wdown[layer]));
     }
-    B2_TRY(upload_matrix(w->ffn_down, kHidden, inter, q8, &st->d_wdown[layer]));
     if (st->layer_kind[layer]) {
         B2_CHECK_ARG(w->fa, "stack_set_layer_weights: layer %d is full attention, fa weights missing", layer);
         std::vector<float> q, k, v, o;
@@ -463,6 +495,9 @@ extern "C" int b200attn_stack_device_status(b200attn_stack st, int* code_out) {
         if (c && !*code_out) *code_out = c;
         return 0;
     }
+    for (const auto* qs : {&st->q8_gu, &st->q8_down})
+        for (auto q : *qs)
+            if (q) { B2_TRY(b200attn_q8_device_status(q, &c)); if (c && !*code_out) *code_out = c; }
     B2_CUDA(cudaDeviceSynchronize());
     B2_CUDA(cudaMemcpy(&c, st->d_error, sizeof(int), cudaMemcpyDeviceToHost));
     if (c) { B2_CUDA(cudaMemset(st->d_error, 0, sizeof(int))); if (!*code_out) *code_out = c; }
@@ -500,11 +535,29 @@ static bool rows_step(b200attn_stack st, int rows) {
     return rows <= kRowsGemmMax && st->cfg.intermediate_size <= 4096 && g_flags.decode_gemm_rows && !gemm_tc_enabled();
 }
 
+// Whether it runs on the tcgen05 projections of gemm_tc.cu, which fold the norms into 16-bit weights.
+static bool tc_step(b200attn_stack st, int rows) { return rows <= 128 && gemm_tc_enabled() && !st->q8_ffn(); }
+
+// h += feed-forward(norm(h)) in 8-bit integers: norm to codes, gate / up with SwiGLU, down from its quantised rows onto h.
+static int stack_ffn_q8(b200attn_stack st, int layer, int rows, cudaStream_t s) {
+    const int inter = st->cfg.intermediate_size;
+    b200attn_norm_args n{};
+    n.rows = rows; n.width = kHidden;
+    n.dtype = B200ATTN_DTYPE_F16; n.x_dtype = B200ATTN_DTYPE_F32;
+    n.d_x = st->d_h; n.ldx = kHidden;
+    n.x_scale = 1.0f; n.eps = st->cfg.rms_eps;
+    n.d_pre_w = st->d_post_norm[layer];
+    n.d_codes = st->d_codes; n.ld_codes = kHidden; n.d_scales = st->d_code_scales;
+    B2_TRY(b200attn_norm_block(&n, s));
+    B2_TRY(b200attn_q8_forward_codes(st->q8_gu[layer], st->d_codes, kHidden, st->d_code_scales, rows, st->d_act, B200ATTN_DTYPE_F16, inter, 0, s));
+    return b200attn_q8_forward(st->q8_down[layer], st->d_act, B200ATTN_DTYPE_F16, inter, rows, st->d_h, B200ATTN_DTYPE_F32, kHidden, 1, st->d_q8_work, st->q8_work_bytes, s);
+}
+
 // All layers over `rows` rows already embedded in d_h (and, for the fused decode step, in d_xh / d_rowsq).
 static int stack_layers(b200attn_stack st, int rows, const int* h_slots, const int* h_counts, int n_seqs, const int* d_slots,
                         bool decode, cudaStream_t s) {
     const int inter = st->cfg.intermediate_size;
-    if (decode && rows <= 128 && gemm_tc_enabled()) {
+    if (decode && tc_step(st, rows)) {
         // Fused decode step, five launches per DeltaNet layer: input projection (RMSNorm scale in its epilogue, the norm's
         // (1 + w) folded into the weights at load), attention, output projection + residual, gate/up + SwiGLU, down +
         // residual.  The residual projections also leave the fp16 copy and the sums of squares the next projection needs.
@@ -532,6 +585,10 @@ static int stack_layers(b200attn_stack st, int rows, const int* h_slots, const i
             else
                 B2_TRY(la_forward_rows(st->la[st->layer_sub[i]], st->state, st->layer_sub[i], h_slots, h_counts, n_seqs, d_slots, true, st->d_h, false,
                                        st->d_h, 1.0f, &f, s));
+            if (st->q8_ffn()) {
+                B2_TRY(stack_ffn_q8(st, i, rows, s));
+                continue;
+            }
             RowsGemm g;
             g.x = st->d_h;
             g.ldx = g.K = kHidden;
@@ -560,6 +617,10 @@ static int stack_layers(b200attn_stack st, int rows, const int* h_slots, const i
         else
             B2_TRY(la_forward_rows(st->la[st->layer_sub[i]], st->state, st->layer_sub[i], h_slots, h_counts, n_seqs, d_slots,
                                    decode, st->d_xb, true, st->d_h, 1.0f, nullptr, s));
+        if (st->q8_ffn()) {
+            B2_TRY(stack_ffn_q8(st, i, rows, s));
+            continue;
+        }
         if (many_rows)
             rmsnorm_rows_kernel<<<ceil_div(rows, 4), 128, 0, s>>>(st->d_h, st->d_post_norm[i], st->cfg.rms_eps, rows, st->d_xb);
         else
@@ -629,7 +690,7 @@ static int stack_decode_layers(b200attn_stack st, int n_seqs, const int* d_token
         if (st->pool) st->pool->lens_marks.mark();
         return block_decode_rows(*st->blocks, n_seqs, d_tokens_in, d_slots, s);
     }
-    if (n_seqs <= 128 && gemm_tc_enabled())
+    if (tc_step(st, n_seqs))
         launch_pdl(embed_gather_fused_kernel, dim3(n_seqs), dim3(256), 0, s, d_tokens_in, st->d_embed, st->cfg.vocab_size, st->d_h, st->d_xh,
                    st->d_rowsq);
     else

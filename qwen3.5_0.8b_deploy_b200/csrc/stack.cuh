@@ -17,6 +17,12 @@ struct b200attn_stack_s {
     std::vector<b200attn_la> la;
     std::vector<float*> d_in_norm, d_post_norm;
     std::vector<__half*> d_wgu, d_wdown;   // [2*inter, hidden], [hidden, inter]
+    std::vector<b200attn_q8> q8_gu, q8_down;   // feed-forward in 8-bit integers (int8_weights 2): in place of these
+    int8_t* d_codes = nullptr;             // [max_rows, hidden] normalised rows in 8 bits, with a scale each
+    float* d_code_scales = nullptr;
+    void* d_q8_work = nullptr;             // of the down projection
+    size_t q8_work_bytes = 0;
+    bool q8_ffn() const { return cfg.int8_weights == 2; }
     std::vector<char> layer_ready;
     __half* d_embed = nullptr;  // [vocab, hidden]
     float* d_final_norm = nullptr;

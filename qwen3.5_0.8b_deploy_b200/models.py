@@ -116,13 +116,14 @@ def build_gutenex(config: dict, limits: Limits, shapes: dict):
 # ---- the hybrid stack: Gated DeltaNet and gated full attention ---------------------------------------------------------------
 @register("Qwen3_5Hybrid")
 def build_hybrid(config: dict, limits: Limits, shapes: dict):
-    """Keys: num_layers, intermediate_size, vocab_size, rms_eps, kv_dtype ("fp16" or "int8"), int8_weights."""
+    """Keys: num_layers, intermediate_size, vocab_size, rms_eps, kv_dtype ("fp16" or "int8"), int8_weights (0, 1, or 2: the feed-forward's products
+    in 8-bit integers too)."""
     ops = _ops()
     if limits.dtype != "bfloat16":
         raise ValueError("the hybrid stack serves 16-bit weights and activations only")
     return ops.HybridStack(config["num_layers"], config["intermediate_size"], config["vocab_size"], limits.max_seqs, limits.max_seq_len,
                            max(1, (limits.max_pass_rows or limits.max_seq_len) // limits.max_seq_len),
-                           ops.KV_INT8 if config.get("kv_dtype") == "int8" else ops.KV_FP16, bool(config.get("int8_weights", False)),
+                           ops.KV_INT8 if config.get("kv_dtype") == "int8" else ops.KV_FP16, int(config.get("int8_weights", 0)),
                            config.get("rms_eps", 1e-6))
 
 

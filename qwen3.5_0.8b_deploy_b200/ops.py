@@ -675,12 +675,12 @@ class Stack:
 
 class HybridStack(Stack):
     """CudaEngine for the attention-facing part: set_layer_weights, forward_batch_prefill,
-    forward_batch_decode, reset_cache, and the captured decode step."""
+    forward_batch_decode, reset_cache, and the captured decode step.  int8_weights 2: the feed-forward in 8-bit integers."""
 
     def __init__(self, num_layers=24, intermediate_size=3584, vocab_size=248320, max_seqs=128, max_seq_len=1536,
                  prefill_chunk_seqs=8, kv_dtype=KV_FP16, int8_weights=True, rms_eps=1e-6):
         self.cfg = StackConfig(num_layers, 1024, intermediate_size, vocab_size, max_seqs, max_seq_len, prefill_chunk_seqs,
-                               kv_dtype, 1 if int8_weights else 0, rms_eps)
+                               kv_dtype, int(int8_weights), rms_eps)
         self.vocab_size, self.max_seqs = vocab_size, max_seqs
         self.h = C.c_void_p()
         _check(_lib.b200attn_stack_create(C.byref(self.cfg), C.byref(self.h)))
