@@ -528,6 +528,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
+    if constexpr (is_q8(EPI)) pdl_launch_dependents();       // small kernels follow: they find room beside this one
 
     // Tiles are numbered along W first: W stays in L2, X passes through once.  The warps that issue loads and products carry stage and parity along
     // and walk their loops whole, with one lane elected for the issue: the chain of instructions of a slice has to stay shorter than its four

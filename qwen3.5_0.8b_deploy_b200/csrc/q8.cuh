@@ -49,6 +49,8 @@ struct Q8Product {
     const void* x = nullptr;         // [rows, in]
     long long ldx = 0;
     ElemType x_type = ELEM_F16;
+    const float* norm_w = nullptr;   // fp32 X of up to 16 short rows (q8_few_rows_quantizes), fp16 Y: X is normalised first, with weights [in]
+    float eps = 0.f;
     const int8_t* codes = nullptr;   // or X as codes, pitch a multiple of 16, and scales
     long long ld_codes = 0;
     const float* scales = nullptr;
@@ -68,5 +70,7 @@ struct Q8Product {
 bool q8_few_rows_takes(int rows, int in);      // the others: gemm_pair_q8, from codes
 bool q8_few_rows_quantizes(int rows, int in, ElemType x_type);       // of those: X need not be codes
 int q8_few_rows(const Q8Product& p, cudaStream_t s);
+// y = q of the normalised rows of x (fp32 [rows, in]), fp16; false where that takes a launch of its own in front.
+bool q8_forward_norm(b200attn_q8 q, const float* x, const float* norm_w, float eps, int rows, __half* y, cudaStream_t s, int* status);
 
 }  // namespace b200

@@ -10,6 +10,7 @@
 #include "q8.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200 {
 namespace {
@@ -75,9 +76,11 @@ constexpr int kUnits = 16, kUnitsShallow = 4;
 __host__ __device__ __forceinline__ int row_share_log2(int rows) { return rows > 8 ? 0 : rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 3 : 4; }    // warps of a row
 inline int units_wanted(int rows, int in, ElemType t) { return ceil_div(ceil_div(in * (int)elem_bytes(t), 512), 1 << row_share_log2(rows)); }
 
-// All rows as codes into shared memory (zeros from column `in` on), their scales beside them.
-template <typename X, int kBatch>
-__device__ __forceinline__ void quantize_rows(const Q8Product& p, int8_t* sx, int pitch, float* s_scale, uint32_t* s_max, int warp, int lane) {
+// All rows as codes into shared memory (zeros from column `in` on), their scales beside them.  kNorm: fp32 rows that are normalised first, as b200attn_norm_block
+// makes codes of them: with the norm's weights (s_norm) multiplied in, and 1 / rms in the scale.
+template <typename X, int kBatch, bool kNorm>
+__device__ __forceinline__ void quantize_rows(const Q8Product& p, int8_t* sx, int pitch, float* s_scale, uint32_t* s_max, float* s_sum, const float* s_norm, int warp,
+                                              int lane) {
     constexpr int kPer = 16 / (int)sizeof(X);
     const int share_log2 = row_share_log2(p.rows), share = 1 << share_log2;
     const int m = warp >> share_log2, sub = warp & (share - 1), step = 32 * kPer * share, first = kPer * (32 * sub + lane);
@@ -87,18 +90,40 @@ __device__ __forceinline__ void quantize_rows(const Q8Product& p, int8_t* sx, in
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) raw[i] = m < p.rows && first + i * step < p.in ? load_unit(row, first + i * step, p.in, aligned) : make_uint4(0, 0, 0, 0);
+    float squares = 0.f;
+    if constexpr (kNorm) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int k = first + i * step;
+            if (k >= p.in) break;
+            float4& x = reinterpret_cast<float4&>(raw[i]);
+            const float4 w = *reinterpret_cast<const float4*>(s_norm + k);
+            squares += (x.x * x.x + x.y * x.y) + (x.z * x.z + x.w * x.w);
+            x = make_float4(__fmul_rn(x.x, w.x), __fmul_rn(x.y, w.y), __fmul_rn(x.z, w.z), __fmul_rn(x.w, w.w));
+        }
+    }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) top = max_unit<X>(top, raw[i]);
     top = max_bits<X>(top);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = 16; o > 0; o >>= 1) {
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (kNorm) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    }
     if (share > 1) {
-        if (lane == 0) s_max[warp] = top;
+        if (lane == 0) {
+            s_max[warp] = top;
+            s_sum[warp] = squares;
+        }
         __syncthreads();
-        for (int i = 0; i < share; ++i) top = max(top, s_max[(m << share_log2) + i]);
+        squares = 0.f;
+        for (int i = 0; i < share; ++i) {
+            top = max(top, s_max[(m << share_log2) + i]);
+            squares += s_sum[(m << share_log2) + i];
+        }
     }
     const Q8Row q = q8_row(top);
-    if (m < p.rows && sub == 0 && lane == 0) s_scale[m] = q.scale;
+    if (m < p.rows && sub == 0 && lane == 0) s_scale[m] = kNorm ? q.scale * (1.0f / sqrtf(squares / (float)p.in + p.eps)) : q.scale;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
         const int k = first + i * step;
@@ -112,13 +137,15 @@ __device__ __forceinline__ void quantize_rows(const Q8Product& p, int8_t* sx, in
 }
 
 // kDeep: all registers of an SM for loads in flight, of weights and of long rows of X.  Otherwise half of them are left to the next launch.
-template <typename X, typename Y, bool kDeep>
+template <typename X, typename Y, bool kDeep, bool kNorm>
 __global__ void __launch_bounds__(kThreads, kDeep ? 1 : 2)
 q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
+    constexpr bool kCodes = std::is_same<X, int8_t>::value;                    // X comes as codes
     constexpr int kAhead = kDeep ? 4 : 2;                                      // blocks of 8 x 128 codes that a warp asks for at once
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float s_scale[kRows];
+    __shared__ float s_scale[kRows], s_wscale[8 * kMostTiles];
     __shared__ uint32_t s_max[kWarps];
+    __shared__ float s_sum[kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pitch = codes_pitch(p.pitch), parts = p.act >= 0 ? 2 : 1;
     int8_t* sx = reinterpret_cast<int8_t*>(smem);
@@ -141,9 +168,19 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
         if (next_c >= c1) { next_c = c0; next_tile += groups; }
     };
     fetch(ring[0]);
+    if constexpr (kCodes) fetch(ring[1]);                                      // X takes the registers otherwise
+    for (int i = threadIdx.x; i < 8 * tiles; i += kThreads) {                  // the scales of this CTA's columns, [part][column]
+        const int part = i >= 8 * (u1 - u0), n = 8 * u0 + i - part * 8 * (u1 - u0);
+        s_wscale[i] = n < p.out ? p.w_scales[part * p.scale_pitch + n] : 0.f;
+    }
+    float* s_norm = reinterpret_cast<float*>(sums + ((size_t)tiles << plan.slices_log2) * 128);
+    if constexpr (kNorm) {
+        for (int i = threadIdx.x; i < p.in; i += kThreads) s_norm[i] = p.norm_w[i];
+        __syncthreads();
+    }
     pdl_launch_dependents();
     pdl_wait();
-    if (p.codes) {
+    if constexpr (kCodes) {
         for (int m = warp; m < kRows; m += kWarps) {
             const int8_t* src = p.codes + m * p.ld_codes;
             for (int k = 16 * lane; k < p.pitch; k += 512)
@@ -151,7 +188,7 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
             if (lane == 0 && m < p.rows) s_scale[m] = p.scales[m];
         }
     } else {
-        quantize_rows<X, kDeep ? kUnits : kUnitsShallow>(p, sx, pitch, s_scale, s_max, warp, lane);
+        quantize_rows<X, kDeep ? kUnits : kUnitsShallow, kNorm>(p, sx, pitch, s_scale, s_max, s_sum, s_norm, warp, lane);
     }
     __syncthreads();
 
@@ -183,10 +220,11 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
         tile += groups;
     };
     while (tile < tiles && c0 < c1) {
-        fetch(ring[1]);
+        if constexpr (!kCodes) fetch(ring[1]);
         multiply(ring[0]);
         fetch(ring[0]);
         multiply(ring[1]);
+        if constexpr (kCodes) fetch(ring[1]);
     }
     __syncthreads();
     const int used = min(slices, (chunks + per - 1) / per);                    // slices with chunks of their own
@@ -198,7 +236,7 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
         for (int part = 0; part < parts; ++part) {
             int sum = 0;
             for (int s = 0; s < used; ++s) sum += sums[(s * tiles + unit * parts + part) * 128 + at];
-            v[part] = (float)sum * s_scale[m] * p.w_scales[part * p.scale_pitch + n];
+            v[part] = (float)sum * s_scale[m] * s_wscale[8 * (part * (u1 - u0) + unit) + (n & 7)];
         }
         if (p.act == B200ATTN_ACT_SILU) v[0] = activated<float, B200ATTN_ACT_SILU>(v[0]) * v[1];
         if (p.act == B200ATTN_ACT_GELU_TANH) v[0] = activated<float, B200ATTN_ACT_GELU_TANH>(v[0]) * v[1];
@@ -210,11 +248,11 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
     }
 }
 
-template <typename X, typename Y, bool kDeep>
+template <typename X, typename Y, bool kDeep, bool kNorm = false>
 int launch_few_rows(const Q8Product& p, const FewPlan& plan, int grid, size_t smem, cudaStream_t s) {
     static PerDeviceOnce once;
-    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024)));
-    launch_pdl_split(true, true, q8_few_rows_kernel<X, Y, kDeep>, dim3(grid), dim3(kThreads), smem, s, p, plan);
+    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep, kNorm>, cudaFuncAttributeMaxDynamicSharedMemorySize, (227 - 4) * 1024)));
+    launch_pdl_split(true, true, q8_few_rows_kernel<X, Y, kDeep, kNorm>, dim3(grid), dim3(kThreads), smem, s, p, plan);
     B2_LAUNCH_CHECK();
     return 0;
 }
@@ -239,17 +277,20 @@ int q8_few_rows(const Q8Product& p, cudaStream_t s) {
         const long long blocks = (long long)ceil_div(tiles, kWarps >> l) * ceil_div(chunks, 1 << l);
         if (l == 0 || blocks < busiest) { busiest = blocks; plan.slices_log2 = l; }
     }
-    const size_t smem = (size_t)kRows * codes_pitch(p.pitch) + ((size_t)tiles << plan.slices_log2) * 512;
+    const size_t smem = (size_t)kRows * codes_pitch(p.pitch) + ((size_t)tiles << plan.slices_log2) * 512 + (p.norm_w ? (size_t)p.in * 4 : 0);
     // More weights than the first fetches of a warp bring in several times over, or long rows of X.  4096 x 2 x 11008 at one row 18.3 us, shallow 21; 1024 x 2 x
     // 3584 at one row 5.4 us, shallow 4.2.
     const bool deep = busiest > 8 || (p.x && units_wanted(p.rows, p.in, p.x_type) > kUnitsShallow);
-    dispatch_elem3(p.x_type, [&](auto xt) {
+    auto launch = [&](auto xt) {
         dispatch_elem3(p.y_type, [&](auto yt) {
             using X = decltype(xt);
             using Y = decltype(yt);
             st = deep ? launch_few_rows<X, Y, true>(p, plan, grid, smem, s) : launch_few_rows<X, Y, false>(p, plan, grid, smem, s);
         });
-    });
+    };
+    if (p.norm_w) return deep ? launch_few_rows<float, __half, true, true>(p, plan, grid, smem, s) : launch_few_rows<float, __half, false, true>(p, plan, grid, smem, s);
+    if (p.codes) launch(int8_t{});
+    else dispatch_elem3(p.x_type, launch);
     return st;
 }
 

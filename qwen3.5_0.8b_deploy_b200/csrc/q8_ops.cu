@@ -66,6 +66,17 @@ int check_output(b200attn_q8 q, const char* what, int rows, const void* d_y, int
 
 }  // namespace
 
+namespace b200 {
+bool q8_forward_norm(b200attn_q8 q, const float* x, const float* norm_w, float eps, int rows, __half* y, cudaStream_t s, int* status) {
+    if (!q8_few_rows_takes(rows, q->in) || !q8_few_rows_quantizes(rows, q->in, ELEM_F32)) return false;
+    Q8Product p = product_of(q, rows, y, q->out, ELEM_F16, 0);
+    p.x = x; p.ldx = q->in; p.x_type = ELEM_F32;
+    p.norm_w = norm_w; p.eps = eps;
+    *status = q8_few_rows(p, s);
+    return true;
+}
+}  // namespace b200
+
 extern "C" int b200attn_q8_quantize(const void* d_x, int dtype, long long ldx, int rows, int cols, int8_t* d_codes, long long ld_codes, float* d_scales,
                                     b200attn_stream stream) {
     ElemType t;

@@ -541,6 +541,12 @@ static bool tc_step(b200attn_stack st, int rows) { return rows <= 128 && gemm_tc
 // h += feed-forward(norm(h)) in 8-bit integers: norm to codes, gate / up with SwiGLU, down from its quantised rows onto h.
 static int stack_ffn_q8(b200attn_stack st, int layer, int rows, cudaStream_t s) {
     const int inter = st->cfg.intermediate_size;
+    int status = 0;
+    if (q8_forward_norm(st->q8_gu[layer], st->d_h, st->d_post_norm[layer], st->cfg.rms_eps, rows, st->d_act, s, &status)) {
+        B2_TRY(status);
+        return b200attn_q8_forward(st->q8_down[layer], st->d_act, B200ATTN_DTYPE_F16, inter, rows, st->d_h, B200ATTN_DTYPE_F32, kHidden, 1, st->d_q8_work,
+                                   st->q8_work_bytes, s);
+    }
     b200attn_norm_args n{};
     n.rows = rows; n.width = kHidden;
     n.dtype = B200ATTN_DTYPE_F16; n.x_dtype = B200ATTN_DTYPE_F32;
