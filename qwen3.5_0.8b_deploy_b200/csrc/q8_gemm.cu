@@ -251,8 +251,10 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
 template <typename X, typename Y, bool kDeep, bool kNorm = false>
 int launch_few_rows(const Q8Product& p, const FewPlan& plan, int grid, size_t smem, cudaStream_t s) {
     static PerDeviceOnce once;
-    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep, kNorm>, cudaFuncAttributeMaxDynamicSharedMemorySize, (227 - 4) * 1024)));
-    launch_pdl_split(true, true, q8_few_rows_kernel<X, Y, kDeep, kNorm>, dim3(grid), dim3(kThreads), smem, s, p, plan);
+    // The split of the L1 store that launch_pdl_split asks for with every launch, which takes the host 1 us each time.
+    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep, kNorm>, cudaFuncAttributeMaxDynamicSharedMemorySize, (227 - 4) * 1024));
+                       B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep, kNorm>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)));
+    launch_pdl(q8_few_rows_kernel<X, Y, kDeep, kNorm>, dim3(grid), dim3(kThreads), smem, s, p, plan);
     B2_LAUNCH_CHECK();
     return 0;
 }

@@ -10,7 +10,6 @@
 // What it took beside the single pass: enough warps to cover the loads (norm to codes at 4 / 5 / 6 blocks of four warps an SM: 111.5 / 110.0 / 119.9 us, the last with
 // spills; the second norm at 1 / 2 / 3 blocks: 143 / 127 / 158), and no branch on the form of the update inside the eight values of a step (130 us).
 #include "elem.cuh"
-#include "gemm_rows.cuh"
 #include "ptx_utils.cuh"
 #include "q8.cuh"
 
@@ -395,9 +394,9 @@ int quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_
         dispatch_run(std::min(run_of(cols, x, ldx, sizeof(T)), run_of(cols, codes, ldc, 1)), [&](auto run) {
             constexpr int kRun = decltype(run)::value;
             if (cols <= 32 * 8 * kQuantGroups)
-                launch_pdl_split(true, rows <= kRowsGemmMax, q8_quantize_kernel<T, true, kRun, kBlocks>, dim3(ceil_div(rows, 4)), dim3(128), 0, s, src, ldx, rows, cols, codes, ldc, scales);
+                launch_pdl(q8_quantize_kernel<T, true, kRun, kBlocks>, dim3(ceil_div(rows, 4)), dim3(128), 0, s, src, ldx, rows, cols, codes, ldc, scales);
             else if (cols <= kBlockThreads * 8 * kQuantGroups)
-                launch_pdl_split(true, rows <= kRowsGemmMax, q8_quantize_kernel<T, false, kRun, kBlocks>, dim3(rows), dim3(threads_for(cols, kQuantGroups)), 0, s, src, ldx, rows, cols, codes, ldc, scales);
+                launch_pdl(q8_quantize_kernel<T, false, kRun, kBlocks>, dim3(rows), dim3(threads_for(cols, kQuantGroups)), 0, s, src, ldx, rows, cols, codes, ldc, scales);
             else
                 launch_pdl(q8_quantize_loop_kernel<T, kBlocks>, dim3(rows), dim3(kLoopThreads), 0, s, src, ldx, cols, codes, ldc, scales);
         });
@@ -408,7 +407,7 @@ int quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_
 
 template <typename X, typename T, int kRun>
 int norm_block(const b200attn_norm_args& a, cudaStream_t s) {
-    const auto wide = [&](auto kernel, int groups) { launch_pdl_split(true, a.rows <= kRowsGemmMax, kernel, dim3(a.rows), dim3(threads_for(a.width, groups)), 0, s, a); };
+    const auto wide = [&](auto kernel, int groups) { launch_pdl(kernel, dim3(a.rows), dim3(threads_for(a.width, groups)), 0, s, a); };
     if (a.width <= 1024 && a.rows > 1024) launch_pdl(norm_block_kernel<X, T, 4, true, kRun>, dim3(ceil_div(a.rows, 4)), dim3(128), 0, s, a);
     else if (a.width <= 4096 && a.rows <= 1024) wide(norm_block_kernel<X, T, 1, false, kRun>, 1);
     else if (a.width <= 8192) wide(norm_block_kernel<X, T, 2, false, kRun>, 2);

@@ -432,7 +432,7 @@ def _matrix(t: torch.Tensor, name: str, cols: int = -1, rows: int = -1, types: d
 def _vector(t: torch.Tensor | None, name: str, n: int) -> int:
     if t is None:
         return 0
-    if t.dtype != torch.float32 or not t.is_cuda or t.get_device() != _device() or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+    if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or not t.is_cuda or t.get_device() != _device():
         raise _invalid(f"{name}: {n} contiguous fp32 values on the current CUDA device wanted")
     return t.data_ptr()
 
@@ -441,13 +441,17 @@ def _current_stream() -> int:
     return _raw_stream(_device())
 
 
+def _rows(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(int8 codes [rows, cols], fp32 scales [rows]) of fp32, fp16 or bf16 rows; x is about codes * scales[:, None].  The codes' row pitch is a
     multiple of 16, as Int8Linear.forward_codes takes it."""
     code, ld = _matrix(x, "quantize_rows")
     rows, cols = x.shape
     pitch = (cols + 15) & -16
-    codes = x.new_empty((rows, pitch), dtype=torch.int8)
+    codes = _rows(rows, pitch, torch.int8, x.device)
     scales = x.new_empty(rows, dtype=torch.float32)
     status = _lib.b200attn_q8_quantize(x.data_ptr(), code, ld, rows, cols, codes.data_ptr(), pitch, scales.data_ptr(), _current_stream())
     if status:
@@ -478,7 +482,7 @@ class Int8Linear:
                 raise _invalid("accumulate wants an output to add to")
             if out_dtype not in _Q8_DTYPES:
                 raise _invalid(f"output type {out_dtype}")
-            return x.new_empty((x.shape[0], self.out_features), dtype=out_dtype), _Q8_DTYPES[out_dtype], self.out_features
+            return _rows(x.shape[0], self.out_features, out_dtype, x.device), _Q8_DTYPES[out_dtype], self.out_features
         return (out, *_matrix(out, "out", self.out_features, x.shape[0]))
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
@@ -568,16 +572,18 @@ def norm_block(x: torch.Tensor, y: torch.Tensor | None = None, pre_w: torch.Tens
         if gate_code != code:
             raise _invalid("gate: the type of y wanted")
         a.d_gate, a.ld_gate, a.gate_kind = gate.data_ptr(), 0 if one else ld, GATE_SIGMOID if sigmoid_gate else GATE_AS_IS
-    a.x_scale, a.y_scale, a.eps = x_scale, y_scale, eps
-    x_out = x if in_place else x.new_empty((rows, width))
+    a.x_scale = x_scale
+    a.y_scale = y_scale
+    a.eps = eps
+    x_out = x if in_place else _rows(rows, width, x.dtype, x.device)
     a.d_x_out, a.ldx_out = x_out.data_ptr(), ldx if in_place else width
     if out_dtype is None:
         pitch = (width + 15) & -16
-        codes, scales = x.new_empty((rows, pitch), dtype=torch.int8), x.new_empty(rows, dtype=torch.float32)
+        codes, scales = _rows(rows, pitch, torch.int8, x.device), x.new_empty(rows, dtype=torch.float32)
         a.d_codes, a.ld_codes, a.d_scales = codes.data_ptr(), pitch, scales.data_ptr()
         result = (x_out, codes if pitch == width else codes[:, :width], scales)
     else:
-        n = x.new_empty((rows, width), dtype=dtype)
+        n = _rows(rows, width, dtype, x.device)
         a.d_out, a.ld_out = n.data_ptr(), width
         result = (x_out, n)
     status = _lib.b200attn_norm_block(C.addressof(a), _current_stream())
