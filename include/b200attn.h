@@ -489,8 +489,9 @@ int b200attn_stack_residual(b200attn_stack st, int rows, float* d_out, int stop_
  * of it is NaN; a row whose largest value is below 2^-116 has the scale 0 and zero codes.
  *
  * Matrices are row-major with a pitch in elements (>= the columns); element types are b200attn_dtype.  Device pointers need the alignment of their
- * element type only.  Rows and columns outside a matrix are neither read nor written.  Except where noted, the calls are asynchronous on `stream`,
- * allocate nothing and may be captured; a call of zero rows does nothing.  Pointers and handles belong to the device that is current.
+ * element type only.  Rows and columns outside a matrix are not written and have no influence.  Outputs overlap no input (but see b200attn_norm_block).
+ * Except where noted, the calls are asynchronous on `stream`, allocate nothing and may be captured; a call of zero rows does nothing.  Pointers and handles
+ * belong to the device that is current.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct b200attn_q8_s* b200attn_q8;   /* weights of an 8-bit product; read-only between calls of set_weights, so that streams may share it */
 
@@ -510,7 +511,7 @@ int b200attn_q8_export(b200attn_q8 q, int8_t* d_codes, float* d_scales, b200attn
  * No reference counterpart. */
 int b200attn_q8_workspace(b200attn_q8 q, int rows, int x_dtype, size_t* bytes_out);
 /* y [rows, out] = x W^T from the codes of x and W: (32-bit integer sum) * row scale * channel scale, or act(gate) * up.  accumulate != 0 (plain
- * fp32 y): added to y.  d_workspace: 16-byte aligned, b200attn_q8_workspace bytes.  x and y must not overlap.  CudaMLP::forward's products
+ * fp32 y): added to y.  d_workspace: 16-byte aligned, b200attn_q8_workspace bytes.  CudaMLP::forward's products
  * (src/backend/cuda/kernels/mlp_cuda.cu:22-39 for the weights); activations in 8 bits have no counterpart. */
 int b200attn_q8_forward(b200attn_q8 q, const void* d_x, int x_dtype, long long ldx, int rows, void* d_y, int y_dtype, long long ldy, int accumulate,
                         void* d_workspace, size_t workspace_bytes, b200attn_stream stream);

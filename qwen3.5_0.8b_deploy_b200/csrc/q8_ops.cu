@@ -19,6 +19,7 @@ struct b200attn_q8_s {
 namespace {
 
 constexpr int kMostIn = 131072;              // 127 * 127 * in < 2^31
+constexpr int kMostRows = INT_MAX - 1023;     // rounded up to whole tiles they are still ints
 constexpr int kPitchStep = 128;              // a slice of the products
 
 bool elem_of(int dtype, ElemType* t) {
@@ -55,7 +56,7 @@ Q8Product product_of(b200attn_q8 q, int rows, void* d_y, long long ldy, ElemType
 }
 
 int check_output(b200attn_q8 q, const char* what, int rows, const void* d_y, int y_dtype, long long ldy, int accumulate, ElemType* yt) {
-    B2_CHECK_ARG(rows >= 0, "%s: negative row count", what);
+    B2_CHECK_ARG(rows >= 0 && rows <= kMostRows, "%s: bad row count %d", what, rows);
     B2_CHECK_ARG(elem_of(y_dtype, yt), "%s: bad output type %d", what, y_dtype);
     B2_CHECK_ARG(rows == 0 || d_y, "%s: null output", what);
     B2_CHECK_ARG(ldy >= q->out, "%s: output pitch %lld below %d columns", what, ldy, q->out);
@@ -81,7 +82,7 @@ extern "C" int b200attn_q8_quantize(const void* d_x, int dtype, long long ldx, i
                                     b200attn_stream stream) {
     ElemType t;
     B2_CHECK_ARG(elem_of(dtype, &t), "q8_quantize: bad element type %d", dtype);
-    B2_CHECK_ARG(rows >= 0 && cols > 0, "q8_quantize: bad sizes %d x %d", rows, cols);
+    B2_CHECK_ARG(rows >= 0 && rows <= kMostRows && cols > 0, "q8_quantize: bad sizes %d x %d", rows, cols);
     B2_CHECK_ARG(ldx >= cols && ld_codes >= cols, "q8_quantize: pitch below %d columns", cols);
     if (rows == 0) return 0;
     B2_CHECK_ARG(d_x && d_codes && d_scales, "q8_quantize: null argument");
@@ -152,7 +153,7 @@ extern "C" int b200attn_q8_export(b200attn_q8 q, int8_t* d_codes, float* d_scale
 
 extern "C" int b200attn_q8_workspace(b200attn_q8 q, int rows, int x_dtype, size_t* bytes_out) {
     ElemType xt;
-    B2_CHECK_ARG(q && bytes_out && rows >= 0, "q8_workspace: bad argument");
+    B2_CHECK_ARG(q && bytes_out && rows >= 0 && rows <= kMostRows, "q8_workspace: bad argument");
     B2_CHECK_ARG(elem_of(x_dtype, &xt), "q8_workspace: bad input type %d", x_dtype);
     *bytes_out = workspace_bytes(q, rows, xt);
     return 0;
@@ -211,7 +212,7 @@ extern "C" int b200attn_norm_block(const b200attn_norm_args* args, b200attn_stre
     ElemType t, xt;
     B2_CHECK_ARG(elem_of(a.dtype, &t) && elem_of(a.x_dtype, &xt), "norm_block: bad element type");
     B2_CHECK_ARG(xt == t || xt == ELEM_F32, "norm_block: x is of the type of y or fp32");
-    B2_CHECK_ARG(a.rows >= 0 && a.width > 0, "norm_block: bad sizes %d x %d", a.rows, a.width);
+    B2_CHECK_ARG(a.rows >= 0 && a.rows <= kMostRows && a.width > 0, "norm_block: bad sizes %d x %d", a.rows, a.width);
     if (a.width > kNormMostWidth) B2_FAIL(B200ATTN_ERR_UNSUPPORTED, "norm_block: width %d above %d", a.width, kNormMostWidth);
     B2_CHECK_ARG(a.ldx >= a.width && (!a.d_y || a.ldy >= a.width) && (!a.d_gate || a.ld_gate == 0 || a.ld_gate >= a.width) &&
                      (!a.d_x_out || a.ldx_out >= a.width) && (!a.d_out || a.ld_out >= a.width) && (!a.d_codes || a.ld_codes >= a.width),

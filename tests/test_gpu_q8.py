@@ -320,7 +320,8 @@ def norm_inputs(rows, width, dtype, x_type, post, gate, pitch=0):
     return x, y, pre, post, g
 
 
-NORM_SIZES = [(1, 1), (1, 1024), (4, 7), (3, 130), (5, 1023), (2, 2050), (9, 4096), (7, 5000), (2, 8192), (3, 8200), (2, 20001), (300, 256), (1, 49152), (66000, 12)]
+NORM_SIZES = [(1, 1), (1, 1024), (4, 7), (3, 130), (5, 1023), (2, 2050), (9, 4096), (7, 5000), (2, 8192), (3, 8200), (2, 20001), (300, 256), (1, 49152), (66000, 12), (1024, 1024), (1025, 1024), (1100, 520), (1030, 1001), (1500, 4096), (1200, 2050),
+              (1100, 10000)]
 
 
 @pytest.mark.parametrize("rows,width", NORM_SIZES)

@@ -18,7 +18,7 @@ def test_quantize_refusals(ops):
     def call(**kw):
         a = dict(ok, **kw)
         return q(a["x"], a["dtype"], a["ldx"], a["rows"], a["cols"], a["codes"], a["ldc"], a["scales"], None)
-    for kw, text in ((dict(dtype=3), b"type"), (dict(dtype=-1), b"type"), (dict(rows=-1), b"sizes"), (dict(cols=0), b"sizes"), (dict(ldx=63), b"pitch"),
+    for kw, text in ((dict(dtype=3), b"type"), (dict(dtype=-1), b"type"), (dict(rows=-1), b"sizes"), (dict(rows=2 ** 31 - 1), b"sizes"), (dict(cols=0), b"sizes"), (dict(ldx=63), b"pitch"),
                      (dict(ldc=63), b"pitch"), (dict(x=None), b"null"), (dict(codes=None), b"null"), (dict(scales=None), b"null"), (dict(x=4097), b"aligned"),
                      (dict(scales=4098), b"aligned"), (dict(dtype=ops.DTYPE_F32, x=4098), b"aligned")):
         refused(ops, call(**kw), text)
