@@ -1,7 +1,7 @@
 // 8-bit operators: row quantiser and norm block (q8_rows.cu), products in 8-bit integers (q8_gemm.cu).
 #pragma once
 
-#include "common.cuh"
+#include "elem.cuh"
 
 namespace b200 {
 
@@ -22,6 +22,18 @@ __device__ __forceinline__ Q8Row q8_row(uint32_t abs_bits) {
 }
 // inv = 0: a zero code, also of a NaN or an infinity (the conversion of a NaN is zero).
 __device__ __forceinline__ int q8_code(float v, float inv) { return __float2int_rn(__fmul_rn(v, inv)); }
+// Largest |value| of words of X: bits of fp32, or of two 16-bit values at a time, which are ordered like the values themselves; q8_max_bits makes bits of fp32 of it.
+template <typename X>
+__device__ __forceinline__ uint32_t q8_max_word(uint32_t top, uint32_t w) {
+    return sizeof(X) == 4 ? max(top, w & 0x7fffffffu) : __vmaxu2(top, w & 0x7fff7fffu);
+}
+template <typename X>
+__device__ __forceinline__ uint32_t q8_max_bits(uint32_t top) {
+    if constexpr (sizeof(X) == 4) return top;
+    const uint16_t bits = (uint16_t)max(top & 0xffffu, top >> 16);
+    return q8_abs_bits(to_f32(*reinterpret_cast<const X*>(&bits)));
+}
+
 // Four codes in the bytes of a word.  1.5 * 2^23 added to a product of at most 127.00001 leaves its nearest integer, ties to even, in the low byte: the same as
 // a conversion, at the rate of additions.
 __device__ __forceinline__ uint32_t q8_codes4(float a, float b, float c, float d, float inv) {

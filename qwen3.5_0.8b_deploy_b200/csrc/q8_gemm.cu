@@ -18,6 +18,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = 16, kRows = 16;
 constexpr int kMostK = 8192;                     // 16 rows of codes in shared memory, and room for the next launch beside them
 constexpr int kMostTiles = 64;                   // of a CTA
+constexpr size_t kMostShared = (227 - 4) * 1024; // of a CTA, beside its static part
 
 struct FewPlan {
     int units;                                   // eights of output columns
@@ -57,19 +58,6 @@ __device__ __forceinline__ void unpack_unit(const uint4& u, float (&v)[16 / size
     for (int j = 0; j < 16 / (int)sizeof(X); ++j) v[j] = to_f32(p[j]);
 }
 
-// Largest |value| of units: bits of fp32, or of two 16-bit values at a time (ordered like the values themselves), which q8_abs_bits makes of the result.
-template <typename X>
-__device__ __forceinline__ uint32_t max_unit(uint32_t top, const uint4& u) {
-    for (const uint32_t w : {u.x, u.y, u.z, u.w}) top = sizeof(X) == 4 ? max(top, w & 0x7fffffffu) : __vmaxu2(top, w & 0x7fff7fffu);
-    return top;
-}
-template <typename X>
-__device__ __forceinline__ uint32_t max_bits(uint32_t top) {
-    if constexpr (sizeof(X) == 4) return top;
-    const uint16_t bits = (uint16_t)max(top & 0xffffu, top >> 16);
-    return q8_abs_bits(to_f32(*reinterpret_cast<const X*>(&bits)));
-}
-
 // Rows of X that lanes hold whole, as so many units each, while they look for the largest value.  Longer ones are quantised by a launch of their own: at 16
 // rows of 8192 fp16 values a CTA would spend more time on them than on its weights (25.7 us against 13.9 for both launches; 16 x 4096 8.1 against 9.2).
 constexpr int kUnits = 16, kUnitsShallow = 4;
@@ -103,8 +91,9 @@ __device__ __forceinline__ void quantize_rows(const Q8Product& p, int8_t* sx, in
         }
     }
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) top = max_unit<X>(top, raw[i]);
-    top = max_bits<X>(top);
+    for (int i = 0; i < kBatch; ++i)
+        for (const uint32_t w : {raw[i].x, raw[i].y, raw[i].z, raw[i].w}) top = q8_max_word<X>(top, w);
+    top = q8_max_bits<X>(top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -123,7 +112,7 @@ __device__ __forceinline__ void quantize_rows(const Q8Product& p, int8_t* sx, in
         }
     }
     const Q8Row q = q8_row(top);
-    if (m < p.rows && sub == 0 && lane == 0) s_scale[m] = kNorm ? q.scale * (1.0f / sqrtf(squares / (float)p.in + p.eps)) : q.scale;
+    if (m < p.rows && sub == 0 && lane == 0) s_scale[m] = kNorm ? q.scale / sqrtf(squares / (float)p.in + p.eps) : q.scale;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
         const int k = first + i * step;
@@ -252,7 +241,7 @@ template <typename X, typename Y, bool kDeep, bool kNorm = false>
 int launch_few_rows(const Q8Product& p, const FewPlan& plan, int grid, size_t smem, cudaStream_t s) {
     static PerDeviceOnce once;
     // The split of the L1 store that launch_pdl_split asks for with every launch, which takes the host 1 us each time.
-    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep, kNorm>, cudaFuncAttributeMaxDynamicSharedMemorySize, (227 - 4) * 1024));
+    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep, kNorm>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared));
                        B2_CUDA(cudaFuncSetAttribute(q8_few_rows_kernel<X, Y, kDeep, kNorm>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)));
     launch_pdl(q8_few_rows_kernel<X, Y, kDeep, kNorm>, dim3(grid), dim3(kThreads), smem, s, p, plan);
     B2_LAUNCH_CHECK();
@@ -280,6 +269,7 @@ int q8_few_rows(const Q8Product& p, cudaStream_t s) {
         if (l == 0 || blocks < busiest) { busiest = blocks; plan.slices_log2 = l; }
     }
     const size_t smem = (size_t)kRows * codes_pitch(p.pitch) + ((size_t)tiles << plan.slices_log2) * 512 + (p.norm_w ? (size_t)p.in * 4 : 0);
+    if (smem > kMostShared) B2_FAIL(B200ATTN_ERR_UNSUPPORTED, "8-bit product: %zu bytes of shared memory for %d rows of %d columns", smem, p.rows, p.in);
     // More weights than the first fetches of a warp bring in several times over, or long rows of X.  4096 x 2 x 11008 at one row 18.3 us, shallow 21; 1024 x 2 x
     // 3584 at one row 5.4 us, shallow 4.2.
     const bool deep = busiest > 8 || (p.x && units_wanted(p.rows, p.in, p.x_type) > kUnitsShallow);

@@ -169,10 +169,11 @@ q8_quantize_kernel(const T* __restrict__ x, long long ldx, int rows, int cols, i
     float v[8];
 #pragma unroll
     for (int i = 0; i < kQuantGroups; ++i) {
-        Eight<kRun>::unpack(raw[i], v);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(raw[i].v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, q8_abs_bits(v[j]));
+        for (int j = 0; j < 2 * (int)sizeof(T); ++j) m = q8_max_word<T>(m, words[j]);
     }
+    m = q8_max_bits<T>(m);
     const Q8Row q = q8_row(row_reduce<kWarp>(m, s_max, RowMax{}));
 #pragma unroll
     for (int i = 0; i < kQuantGroups; ++i) {
@@ -233,7 +234,7 @@ __device__ __forceinline__ void norm_update(const b200attn_norm_args& a, float (
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = __fadd_rn(x[j], __fmul_rn(y[j], a.y_scale));
 }
-__device__ __forceinline__ float norm_factor(float squares, const b200attn_norm_args& a) { return 1.0f / sqrtf(squares / (float)a.width + a.eps); }
+__device__ __forceinline__ float norm_rms(float squares, const b200attn_norm_args& a) { return sqrtf(squares / (float)a.width + a.eps); }
 
 template <typename X, typename T, int kGroups, bool kWarp, int kRun>
 __global__ void __launch_bounds__(kWarp ? 128 : kBlockThreads, kRun < 8 ? 1 : kWarp ? 5 : kGroups > 2 ? 1 : 2)
@@ -272,7 +273,7 @@ norm_block_kernel(const b200attn_norm_args a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss += z[j] * z[j];
         }
-        post = norm_factor(row_reduce<kWarp>(ss, s_post, RowSum{}), a);
+        post = 1.0f / norm_rms(row_reduce<kWarp>(ss, s_post, RowSum{}), a);
         ss = 0.f;
     }
     uint32_t m = 0;
@@ -303,11 +304,11 @@ norm_block_kernel(const b200attn_norm_args a) {
         }
     }
     if (!a.d_out && !a.d_codes) return;
-    const float pre = norm_factor(row_reduce<kWarp>(ss, s_pre, RowSum{}), a);
+    const float rms = norm_rms(row_reduce<kWarp>(ss, s_pre, RowSum{}), a), pre = 1.0f / rms;
     Q8Row q{};
     if (a.d_codes) {
         q = q8_row(row_reduce<kWarp>(m, s_max, RowMax{}));
-        if (t == 0) a.d_scales[row] = q.scale * pre;
+        if (t == 0) a.d_scales[row] = q.scale / rms;
     }
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
@@ -339,7 +340,7 @@ norm_block_loop_kernel(const b200attn_norm_args a) {
     if (a.d_post_w) {
         float ss = 0.f;
         for (int c = threadIdx.x; c < a.width; c += kLoopThreads) { const float v = to_f32(y[c]); ss += v * v; }
-        post = norm_factor(row_reduce<false>(ss, s_post, RowSum{}), a);
+        post = 1.0f / norm_rms(row_reduce<false>(ss, s_post, RowSum{}), a);
     }
     float ss = 0.f;
     uint32_t m = 0;
@@ -355,7 +356,7 @@ norm_block_loop_kernel(const b200attn_norm_args a) {
         s_row[c] = v;
     }
     if (!a.d_out && !a.d_codes) return;
-    const float pre = norm_factor(row_reduce<false>(ss, s_pre, RowSum{}), a);
+    const float rms = norm_rms(row_reduce<false>(ss, s_pre, RowSum{}), a), pre = 1.0f / rms;
     if (a.d_out) {
         T* out = static_cast<T*>(a.d_out) + row * a.ld_out;
         for (int c = threadIdx.x; c < a.width; c += kLoopThreads) out[c] = from_f32<T>(s_row[c] * pre);
@@ -364,7 +365,7 @@ norm_block_loop_kernel(const b200attn_norm_args a) {
         const Q8Row q = q8_row(row_reduce<false>(m, s_max, RowMax{}));
         int8_t* codes = a.d_codes + row * a.ld_codes;
         for (int c = threadIdx.x; c < a.width; c += kLoopThreads) codes[c] = (int8_t)q8_code(s_row[c], q.inv);
-        if (threadIdx.x == 0) a.d_scales[row] = q.scale * pre;
+        if (threadIdx.x == 0) a.d_scales[row] = q.scale / rms;
     }
 }
 

@@ -472,6 +472,7 @@ class Int8Linear:
             if _matrix(w, "up", self.in_features, self.out_features) != (code, ld):
                 raise _invalid("gate and up: the same element type and row pitch wanted")
         self.act = act
+        self._sized = (0, 0, 0)        # the last call's rows and type, and the workspace that they want
         self.h = C.c_void_p()
         _check(_lib.b200attn_q8_create(C.c_int(self.out_features), C.c_int(self.in_features), C.c_int(act), C.byref(self.h)))
         _check(_lib.b200attn_q8_set_weights(self.h, weights[0].data_ptr(), weights[1].data_ptr() if act >= 0 else None, code, ld, _current_stream()))
@@ -490,11 +491,15 @@ class Int8Linear:
         code, ld = _matrix(x, "x", self.in_features)
         out, out_code, out_ld = self._output(x, out_dtype or x.dtype, out, accumulate)
         rows = x.shape[0]
-        n = C.c_size_t(0)
-        status = _lib.b200attn_q8_workspace(self.h, rows, code, C.byref(n))
-        ws = x.new_empty(n.value, dtype=torch.uint8) if n.value else None
-        status = status or _lib.b200attn_q8_forward(self.h, x.data_ptr(), code, ld, rows, out.data_ptr(), out_code, out_ld, accumulate,
-                                                    ws.data_ptr() if n.value else None, n.value, _current_stream())
+        sized = self._sized
+        if sized[0] != rows or sized[1] != code:
+            n = C.c_size_t(0)
+            _check(_lib.b200attn_q8_workspace(self.h, rows, code, C.byref(n)))
+            self._sized = sized = (rows, code, n.value)
+        n = sized[2]
+        ws = x.new_empty(n, dtype=torch.uint8) if n else None          # of this call: calls on other streams have theirs
+        status = _lib.b200attn_q8_forward(self.h, x.data_ptr(), code, ld, rows, out.data_ptr(), out_code, out_ld, accumulate, ws.data_ptr() if n else None, n,
+                                          _current_stream())
         if status:
             _check(status)
         return out

@@ -138,7 +138,7 @@ def glu_bound(g, u, act, dtype):
 
 SIZES = [(1, 64, 8), (1, 1, 1), (2, 17, 3), (1, 1024, 3584), (3, 1000, 2313), (16, 4096, 515), (15, 128, 64), (16, 7, 40), (17, 256, 96), (31, 1024, 129), (33, 130, 1000),
          (64, 2048, 256), (100, 999, 257), (128, 1024, 1024), (129, 72, 33), (255, 512, 640), (257, 384, 2000), (300, 8192, 31), (777, 1003, 511), (1025, 640, 300), (4, 12000, 90),
-         (2000, 100, 1), (513, 33, 7), (7, 6000, 1000), (40, 20000, 50), (11, 20000, 50), (2, 131072, 9), (18, 131072, 9), (16, 8192, 100), (9, 4096, 70), (16, 2048, 30), (8, 8192, 60), (4, 8191, 50), (1, 8192, 4100)]
+         (2000, 100, 1), (513, 33, 7), (7, 6000, 1000), (40, 20000, 50), (11, 20000, 50), (2, 131072, 9), (18, 131072, 9), (16, 8192, 100), (9, 4096, 70), (16, 2048, 30), (8, 8192, 60), (4, 8191, 50), (1, 8192, 4100), (2, 40, 100003), (20, 40, 50001)]
 
 
 @pytest.mark.parametrize("rows,cols,out", SIZES)

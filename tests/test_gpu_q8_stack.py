@@ -78,10 +78,12 @@ def test_prompts(ops, cuda, synth, seqs, tokens, chunk):
         assert (err <= 16 * 2.0 ** -23 * want.abs()).all(), (err / want.abs()).max()
 
 
-@pytest.mark.parametrize("rows", [1, 4, 16, 17, 40, 130])
-def test_decode_steps(ops, cuda, synth, rows):
-    """Eager and captured steps, few rows (up to 16) and more."""
+@pytest.mark.parametrize("rows,gemm", [(1, ""), (4, ""), (16, ""), (17, ""), (40, ""), (130, ""), (3, "tc"), (20, "tc"), (3, "cublas"), (20, "cublas")])
+def test_decode_steps(ops, cuda, synth, monkeypatch, rows, gemm):
+    """Eager and captured steps, few rows (up to 16) and more, under every choice of the other projections' kernels."""
     torch = cuda
+    if gemm:
+        monkeypatch.setenv("B200ATTN_DECODE_GEMM", gemm)
     w = make(synth, 90 + rows, True)
     st, ref = build(ops, w, rows, 16, 1), Reference(cuda, ops, w)
     toks = torch.from_numpy(synth.rng(6, "q8.tokens").integers(0, VOCAB, (rows,)).astype(np.int32)).cuda()
