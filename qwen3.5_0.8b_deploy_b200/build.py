@@ -70,7 +70,35 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
 def build(force: bool = False, verbose: bool = False) -> str:
     build_library(force, verbose)
     build_compat(force)
+    build_binding(force)
     return OUT
+
+
+def build_binding(force: bool = False) -> None:
+    """_q8.so, the Python calls of the 8-bit operators (csrc/q8_python.cpp): on PyTorch's C++ API, beside the library it calls."""
+    import sysconfig
+
+    import torch
+    src, out = os.path.join(CSRC, "q8_python.cpp"), os.path.join(HERE, "_q8.so")
+    header = os.path.join(HERE, "..", "include", "b200attn.h")
+    # by the interpreter and the PyTorch it was built for too: their interfaces are not the next version's
+    made_for = f"{sys.version} {torch.__version__}"
+    mark = os.path.join(OBJ, "q8_python.for")
+    if not force and os.path.exists(out) and os.path.getmtime(out) > max(os.path.getmtime(src), os.path.getmtime(header)) and \
+            os.path.exists(mark) and open(mark).read() == made_for:
+        return
+    os.makedirs(OBJ, exist_ok=True)
+    where = os.path.dirname(torch.__file__)
+    part = f"{out}.{os.getpid()}"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{where}/include", "-I/usr/local/cuda/include", src, "-o", part, f"-L{HERE}", "-lb200attn",
+           f"-L{where}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{where}/lib"]
+    p = subprocess.run(cmd, capture_output=True, text=True)
+    if p.returncode != 0:
+        raise RuntimeError(f"binding build failed: {' '.join(cmd)}\n{p.stderr[-4000:]}")
+    os.replace(part, out)
+    with open(mark, "w") as f:
+        f.write(made_for)
 
 
 def build_compat(force: bool = False) -> None:

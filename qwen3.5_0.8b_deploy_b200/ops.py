@@ -9,6 +9,7 @@ raises: there is no fallback path.
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 import os
 
 import numpy as np
@@ -402,7 +403,28 @@ class LinearAttention:
 
 
 # ---- feed-forward in 8-bit integers ------------------------------------------------------------------------------------
-# A call of a few rows takes the GPU 2 to 4 us, so the checks here are kept short: one pass over what a good call has, reasons only for a bad one.
+# The calls of a pass (quantize_rows, forward, forward_codes, norm_block) are in csrc/q8_python.cpp, checks of their tensors included: products of a few rows
+# take the GPU 2 to 4 us, less than the same steps take in Python.  They go through the same C ABI.
+_binding = None
+
+
+def _q8_fail(status: int, message: str) -> None:
+    raise (InvalidArgument if status == ERR_INVALID else B200AttnError)(status, message)
+
+
+def _native():
+    global _binding
+    if _binding is None:
+        try:
+            module = importlib.import_module("._q8", __package__)
+        except ImportError as e:
+            raise ImportError(f"{os.path.join(_HERE, '_q8.so')} is missing or was built for another Python or PyTorch: build it with "
+                              "`python __graft_entry__.py build`") from e
+        module.set_fail(_q8_fail)
+        _binding = module
+    return _binding
+
+
 _Q8_DTYPES = {torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32, torch.float16: DTYPE_F16}
 _device = getattr(torch._C, "_cuda_getDevice", None)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -429,34 +451,14 @@ def _matrix(t: torch.Tensor, name: str, cols: int = -1, rows: int = -1, types: d
     raise _invalid(f"{name}: shape {tuple(shape)}, wanted [{rows if rows >= 0 else 'rows'}, {cols if cols >= 0 else 'columns'}]")
 
 
-def _vector(t: torch.Tensor | None, name: str, n: int) -> int:
-    if t is None:
-        return 0
-    if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or not t.is_cuda or t.get_device() != _device():
-        raise _invalid(f"{name}: {n} contiguous fp32 values on the current CUDA device wanted")
-    return t.data_ptr()
-
-
 def _current_stream() -> int:
     return _raw_stream(_device())
-
-
-def _rows(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
-    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(int8 codes [rows, cols], fp32 scales [rows]) of fp32, fp16 or bf16 rows; x is about codes * scales[:, None].  The codes' row pitch is a
     multiple of 16, as Int8Linear.forward_codes takes it."""
-    code, ld = _matrix(x, "quantize_rows")
-    rows, cols = x.shape
-    pitch = (cols + 15) & -16
-    codes = _rows(rows, pitch, torch.int8, x.device)
-    scales = x.new_empty(rows, dtype=torch.float32)
-    status = _lib.b200attn_q8_quantize(x.data_ptr(), code, ld, rows, cols, codes.data_ptr(), pitch, scales.data_ptr(), _current_stream())
-    if status:
-        _check(status)
-    return (codes if pitch == cols else codes[:, :cols]), scales
+    return (_binding or _native()).quantize_rows(x)
 
 
 class Int8Linear:
@@ -472,51 +474,19 @@ class Int8Linear:
             if _matrix(w, "up", self.in_features, self.out_features) != (code, ld):
                 raise _invalid("gate and up: the same element type and row pitch wanted")
         self.act = act
-        self._sized = (0, 0, 0)        # the last call's rows and type, and the workspace that they want
         self.h = C.c_void_p()
         _check(_lib.b200attn_q8_create(C.c_int(self.out_features), C.c_int(self.in_features), C.c_int(act), C.byref(self.h)))
         _check(_lib.b200attn_q8_set_weights(self.h, weights[0].data_ptr(), weights[1].data_ptr() if act >= 0 else None, code, ld, _current_stream()))
-
-    def _output(self, x: torch.Tensor, out_dtype, out, accumulate: bool) -> tuple[torch.Tensor, int, int]:
-        if out is None:
-            if accumulate:
-                raise _invalid("accumulate wants an output to add to")
-            if out_dtype not in _Q8_DTYPES:
-                raise _invalid(f"output type {out_dtype}")
-            return _rows(x.shape[0], self.out_features, out_dtype, x.device), _Q8_DTYPES[out_dtype], self.out_features
-        return (out, *_matrix(out, "out", self.out_features, x.shape[0]))
+        self._args = (self.h.value, self.in_features, self.out_features)
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
         """[rows, in] -> [rows, out] of out_dtype (default: x's), into `out` if given (fp32 and accumulate: added to it)."""
-        code, ld = _matrix(x, "x", self.in_features)
-        out, out_code, out_ld = self._output(x, out_dtype or x.dtype, out, accumulate)
-        rows = x.shape[0]
-        sized = self._sized
-        if sized[0] != rows or sized[1] != code:
-            n = C.c_size_t(0)
-            _check(_lib.b200attn_q8_workspace(self.h, rows, code, C.byref(n)))
-            self._sized = sized = (rows, code, n.value)
-        n = sized[2]
-        ws = x.new_empty(n, dtype=torch.uint8) if n else None          # of this call: calls on other streams have theirs
-        status = _lib.b200attn_q8_forward(self.h, x.data_ptr(), code, ld, rows, out.data_ptr(), out_code, out_ld, accumulate, ws.data_ptr() if n else None, n,
-                                          _current_stream())
-        if status:
-            _check(status)
-        return out
+        return (_binding or _native()).forward(*self._args, x, out_dtype, out, accumulate)
 
     def forward_codes(self, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
                       accumulate: bool = False) -> torch.Tensor:
         """The same from what quantize_rows or norm_block returned."""
-        _, ld = _matrix(codes, "codes", self.in_features, types={torch.int8: 0})
-        out, out_code, out_ld = self._output(codes, out_dtype, out, accumulate)
-        rows = codes.shape[0]
-        if rows <= 1:
-            ld = (ld + 15) & -16          # one row, which may come without the pitch of a matrix
-        status = _lib.b200attn_q8_forward_codes(self.h, codes.data_ptr(), ld, _vector(scales, "scales", rows), rows, out.data_ptr(), out_code, out_ld,
-                                                accumulate, _current_stream())
-        if status:
-            _check(status)
-        return out
+        return (_binding or _native()).forward_codes(*self._args, codes, scales, out_dtype, out, accumulate)
 
     def weight_codes(self) -> tuple[torch.Tensor, torch.Tensor]:
         """Codes and scales of the weights, a gated pair's gate rows in front of its up rows."""
@@ -556,45 +526,7 @@ def norm_block(x: torch.Tensor, y: torch.Tensor | None = None, pre_w: torch.Tens
     y is None (no block output yet) or of the activations' type; post_w None leaves its norm out; gate is [rows, width], [width] or None.  Returns
     (x', n) with n of `out_dtype` (y's type where there is a y), or (x', codes, scales) when out_dtype is None.  in_place: x' is x.
     """
-    x_code, ldx = _matrix(x, "x")
-    rows, width = x.shape
-    dtype = y.dtype if y is not None else out_dtype or x.dtype
-    code = _Q8_DTYPES.get(dtype)
-    if code is None or (out_dtype is not None and out_dtype != dtype):
-        raise _invalid(f"norm_block: output type {out_dtype} for activations of {dtype}")
-    a = NormArgs(rows, width, code, x_code, x.data_ptr(), ldx)
-    if y is not None:
-        a.d_y = y.data_ptr()
-        a.ldy = _matrix(y, "y", width, rows)[1]
-    if post_w is not None:
-        a.d_post_w = _vector(post_w, "post_w", width)
-    if pre_w is not None:
-        a.d_pre_w = _vector(pre_w, "pre_w", width)
-    if gate is not None:
-        one = gate.dim() == 1
-        gate = gate[None] if one else gate
-        gate_code, ld = _matrix(gate, "gate", width, 1 if one else rows)
-        if gate_code != code:
-            raise _invalid("gate: the type of y wanted")
-        a.d_gate, a.ld_gate, a.gate_kind = gate.data_ptr(), 0 if one else ld, GATE_SIGMOID if sigmoid_gate else GATE_AS_IS
-    a.x_scale = x_scale
-    a.y_scale = y_scale
-    a.eps = eps
-    x_out = x if in_place else _rows(rows, width, x.dtype, x.device)
-    a.d_x_out, a.ldx_out = x_out.data_ptr(), ldx if in_place else width
-    if out_dtype is None:
-        pitch = (width + 15) & -16
-        codes, scales = _rows(rows, pitch, torch.int8, x.device), x.new_empty(rows, dtype=torch.float32)
-        a.d_codes, a.ld_codes, a.d_scales = codes.data_ptr(), pitch, scales.data_ptr()
-        result = (x_out, codes if pitch == width else codes[:, :width], scales)
-    else:
-        n = _rows(rows, width, dtype, x.device)
-        a.d_out, a.ld_out = n.data_ptr(), width
-        result = (x_out, n)
-    status = _lib.b200attn_norm_block(C.addressof(a), _current_stream())
-    if status:
-        _check(status)
-    return result
+    return (_binding or _native()).norm_block(x, y, pre_w, post_w, gate, sigmoid_gate, x_scale, y_scale, eps, out_dtype, in_place)
 
 
 # ---- hybrid stack + graph-captured decode -------------------------------------------------------------------------
