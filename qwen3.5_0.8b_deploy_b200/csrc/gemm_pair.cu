@@ -505,8 +505,11 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
         }
         mbar_init(acc_full(0), 1);
         mbar_init(acc_full(1), 1);
-        mbar_init(acc_empty(0), 2 * Smem::kReaders);
-        mbar_init(acc_empty(1), 2 * Smem::kReaders);
+        // 8-bit products: the epilogue warps signal in their own CTA, and the neighbour's last warp passes it on.  A release to the other CTA waits for the
+        // arriving thread's stores, which of an epilogue warp are its results on their way to memory.
+        const int readers = !is_q8(EPI) ? 2 * Smem::kReaders : rank == 0 ? Smem::kReaders + 1 : Smem::kReaders;
+        mbar_init(acc_empty(0), readers);
+        mbar_init(acc_empty(1), readers);
         mbar_init(halted, 1);
         *abort_flag = 0;
         mbar_fence_init();
@@ -608,6 +611,15 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
                 if (elect_one()) umma_commit_pair(halted, 1);
                 mbar_drain(halted, 0);
             }
+        } else if constexpr (is_q8(EPI)) {
+            int i = 0;
+            for (int t = pair; t < p.items; t += pairs, ++i) {
+                if (!mbar_wait_warp<kClusterScope>(acc_empty(i & 1), (i >> 1) & 1, abort_flag)) break;
+                tc_fence_after();
+                tc_fence_before();
+                if (lane == 0) mbar_arrive_cluster(cluster_smem_addr(acc_empty(i & 1), 0));
+                __syncwarp();
+            }
         }
     } else {
         const int q = warp & 3, part = warp >> 2;          // TMEM lanes 32 q .. 32 q + 31, a quarter of the columns
@@ -672,7 +684,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
                     auto early = [&] {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster_relaxed(cluster_smem_addr(acc_empty(b), 0));
+                        if (lane == 0) mbar_arrive(acc_empty(b));
                     };
                     if (q8_mine) q8_part<EPI, T, kAct>(p, &maps.out[0], first_col, second_col, scales, out_smem, out, q8_row(w), q8_col(w), sx, lane, early);
                     else early();

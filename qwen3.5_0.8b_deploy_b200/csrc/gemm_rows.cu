@@ -94,15 +94,6 @@ __device__ __forceinline__ float rows_act(float g) {
     else return times_sigmoid<A>(g, g);
 }
 
-// The next kernel of the stream may take its place at once.  If it is one of these it fetches weights and waits; any other waits before it touches
-// what a step writes, or reads recurrent state that was written before the step's embedding launch, which waits first (la_decode_kernel).  Where no
-// such launch lies between two calls (RowsGemm::late) this one waits first, whichever of the kernels the shape takes.
-__device__ __forceinline__ void rows_enter(bool late) {
-    if (!late) pdl_launch_dependents();
-    pdl_wait();
-    if (late) pdl_launch_dependents();
-}
-
 constexpr int kRowsThreads = 512, kRowsWarps = 16, kRows = kRowsGemmMax;
 static_assert(kRows == 16, "one row tile of mma.m16n8k16");
 

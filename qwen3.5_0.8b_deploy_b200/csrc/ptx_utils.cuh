@@ -113,10 +113,6 @@ __device__ __forceinline__ uint32_t cluster_smem_addr(uint32_t local_smem_addr, 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// The same without the wait for this thread's earlier stores, where nothing that was written is handed over.
-__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
 
 // Every thread of every CTA of the cluster (threads that have exited do not count).
 __device__ __forceinline__ void cluster_sync_all() {
@@ -157,6 +153,14 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_enter() { pdl_wait(); pdl_launch_dependents(); }
+// Products of few rows in a decode step: the next kernel of the stream may take its place at once.  If it is one of these it fetches weights and waits; any other
+// waits before it touches what a step writes, or reads recurrent state that was written before the step's embedding launch, which waits first
+// (la_decode_kernel).  Where no such launch lies between two calls (late) this one waits first, whichever of the kernels the shape takes.
+__device__ __forceinline__ void rows_enter(bool late) {
+    if (!late) pdl_launch_dependents();
+    pdl_wait();
+    if (late) pdl_launch_dependents();
+}
 
 // Hint: bring `bytes` (a multiple of 16, 16-byte aligned source) into L2; nothing waits for it.
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {

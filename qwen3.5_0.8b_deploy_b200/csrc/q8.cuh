@@ -78,11 +78,13 @@ struct Q8Product {
     ElemType y_type = ELEM_F32;
     bool accumulate = false;         // fp32 Y: added to what is there
     int* error = nullptr;
+    bool late = true;                // few rows: the next launch is let in behind the wait (rows_enter)
 };
 bool q8_few_rows_takes(int rows, int in);      // the others: gemm_pair_q8, from codes
 bool q8_few_rows_quantizes(int rows, int in, ElemType x_type);       // of those: X need not be codes
 int q8_few_rows(const Q8Product& p, cudaStream_t s);
-// y = q of the normalised rows of x (fp32 [rows, in]), fp16; false where that takes a launch of its own in front.
-bool q8_forward_norm(b200attn_q8 q, const float* x, const float* norm_w, float eps, int rows, __half* y, cudaStream_t s, int* status);
+// The products of a decode step of few rows, a single launch each; false where they take more.  y = q of the normalised rows of x, fp16; y += q of fp16 x.
+bool q8_step_norm(b200attn_q8 q, const float* x, const float* norm_w, float eps, int rows, __half* y, cudaStream_t s, int* status);
+bool q8_step_residual(b200attn_q8 q, const __half* x, int rows, float* y, cudaStream_t s, int* status);
 
 }  // namespace b200

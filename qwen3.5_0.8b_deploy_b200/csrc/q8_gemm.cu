@@ -146,7 +146,7 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
 
     Weights ring[2][kAhead];
     int next_tile = group, next_c = c0;                                        // what is asked for next
-    auto fetch = [&](Weights (&b)[kAhead]) {
+    auto fetch = [&](auto& b) {
         if (next_tile >= tiles || c0 >= c1) return;
         const int unit = u0 + (parts == 2 ? next_tile >> 1 : next_tile), row = 8 * unit + (parts == 2 && next_tile & 1 ? p.up_row : 0);
         const int8_t* w = p.w + (long long)row * p.pitch + next_c * kQ8Block + 32 * lane;
@@ -167,8 +167,7 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
         for (int i = threadIdx.x; i < p.in; i += kThreads) s_norm[i] = p.norm_w[i];
         __syncthreads();
     }
-    pdl_launch_dependents();
-    pdl_wait();
+    rows_enter(p.late);
     if constexpr (kCodes) {
         for (int m = warp; m < kRows; m += kWarps) {
             const int8_t* src = p.codes + m * p.ld_codes;
@@ -184,7 +183,7 @@ q8_few_rows_kernel(const Q8Product p, const FewPlan plan) {
     const bool high = p.rows > 8;
     const int8_t* xp = sx + g * pitch + 32 * t;
     int acc[4] = {0, 0, 0, 0}, tile = group, c = c0;
-    auto multiply = [&](const Weights (&b)[kAhead]) {
+    auto multiply = [&](const auto& b) {
         if (tile >= tiles || c0 >= c1) return;
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)

@@ -68,13 +68,20 @@ int check_output(b200attn_q8 q, const char* what, int rows, const void* d_y, int
 }  // namespace
 
 namespace b200 {
-bool q8_forward_norm(b200attn_q8 q, const float* x, const float* norm_w, float eps, int rows, __half* y, cudaStream_t s, int* status) {
-    if (!q8_few_rows_takes(rows, q->in) || !q8_few_rows_quantizes(rows, q->in, ELEM_F32)) return false;
-    Q8Product p = product_of(q, rows, y, q->out, ELEM_F16, 0);
-    p.x = x; p.ldx = q->in; p.x_type = ELEM_F32;
-    p.norm_w = norm_w; p.eps = eps;
+static bool q8_step(b200attn_q8 q, Q8Product p, const void* x, ElemType x_type, cudaStream_t s, int* status) {
+    if (!q8_few_rows_takes(p.rows, q->in) || !q8_few_rows_quantizes(p.rows, q->in, x_type)) return false;
+    p.x = x; p.ldx = q->in; p.x_type = x_type;
+    p.late = false;
     *status = q8_few_rows(p, s);
     return true;
+}
+bool q8_step_norm(b200attn_q8 q, const float* x, const float* norm_w, float eps, int rows, __half* y, cudaStream_t s, int* status) {
+    Q8Product p = product_of(q, rows, y, q->out, ELEM_F16, 0);
+    p.norm_w = norm_w; p.eps = eps;
+    return q8_step(q, p, x, ELEM_F32, s, status);
+}
+bool q8_step_residual(b200attn_q8 q, const __half* x, int rows, float* y, cudaStream_t s, int* status) {
+    return q8_step(q, product_of(q, rows, y, q->out, ELEM_F32, 1), x, ELEM_F16, s, status);
 }
 }  // namespace b200
 

@@ -538,12 +538,14 @@ static bool rows_step(b200attn_stack st, int rows) {
 // Whether it runs on the tcgen05 projections of gemm_tc.cu, which fold the norms into 16-bit weights.
 static bool tc_step(b200attn_stack st, int rows) { return rows <= 128 && gemm_tc_enabled() && !st->q8_ffn(); }
 
-// h += feed-forward(norm(h)) in 8-bit integers: norm to codes, gate / up with SwiGLU, down from its quantised rows onto h.
-static int stack_ffn_q8(b200attn_stack st, int layer, int rows, cudaStream_t s) {
+// h += feed-forward(norm(h)) in 8-bit integers: norm to codes, gate / up with SwiGLU, down from its quantised rows onto h.  In decode steps of few rows the
+// products normalise and quantise for themselves.
+static int stack_ffn_q8(b200attn_stack st, int layer, int rows, bool decode, cudaStream_t s) {
     const int inter = st->cfg.intermediate_size;
     int status = 0;
-    if (q8_forward_norm(st->q8_gu[layer], st->d_h, st->d_post_norm[layer], st->cfg.rms_eps, rows, st->d_act, s, &status)) {
+    if (decode && q8_step_norm(st->q8_gu[layer], st->d_h, st->d_post_norm[layer], st->cfg.rms_eps, rows, st->d_act, s, &status)) {
         B2_TRY(status);
+        if (q8_step_residual(st->q8_down[layer], st->d_act, rows, st->d_h, s, &status)) return status;
         return b200attn_q8_forward(st->q8_down[layer], st->d_act, B200ATTN_DTYPE_F16, inter, rows, st->d_h, B200ATTN_DTYPE_F32, kHidden, 1, st->d_q8_work,
                                    st->q8_work_bytes, s);
     }
@@ -592,7 +594,7 @@ static int stack_layers(b200attn_stack st, int rows, const int* h_slots, const i
                 B2_TRY(la_forward_rows(st->la[st->layer_sub[i]], st->state, st->layer_sub[i], h_slots, h_counts, n_seqs, d_slots, true, st->d_h, false,
                                        st->d_h, 1.0f, &f, s));
             if (st->q8_ffn()) {
-                B2_TRY(stack_ffn_q8(st, i, rows, s));
+                B2_TRY(stack_ffn_q8(st, i, rows, true, s));
                 continue;
             }
             RowsGemm g;
@@ -624,7 +626,7 @@ static int stack_layers(b200attn_stack st, int rows, const int* h_slots, const i
             B2_TRY(la_forward_rows(st->la[st->layer_sub[i]], st->state, st->layer_sub[i], h_slots, h_counts, n_seqs, d_slots,
                                    decode, st->d_xb, true, st->d_h, 1.0f, nullptr, s));
         if (st->q8_ffn()) {
-            B2_TRY(stack_ffn_q8(st, i, rows, s));
+            B2_TRY(stack_ffn_q8(st, i, rows, decode, s));
             continue;
         }
         if (many_rows)
