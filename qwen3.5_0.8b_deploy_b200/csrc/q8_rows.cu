@@ -409,8 +409,13 @@ int quantize(ElemType t, const void* x, long long ldx, int rows, int cols, int8_
 template <typename X, typename T, int kRun>
 int norm_block(const b200attn_norm_args& a, cudaStream_t s) {
     const auto wide = [&](auto kernel, int groups) { launch_pdl(kernel, dim3(a.rows), dim3(threads_for(a.width, groups)), 0, s, a); };
-    if (a.width <= 1024 && a.rows > 1024) launch_pdl(norm_block_kernel<X, T, 4, true, kRun>, dim3(ceil_div(a.rows, 4)), dim3(128), 0, s, a);
-    else if (a.width <= 4096 && a.rows <= 1024) wide(norm_block_kernel<X, T, 1, false, kRun>, 1);
+    // A thread per eight values as long as all rows are under way at once with them (64 registers each), else fewer threads that have more to wait for: 1000 x 4096
+    // 10.3 us, with 512 threads a row 13.5.  Values one by one or in pairs keep more threads busy: 777 x 2050 8.4 us, with two eights a thread 10.4.
+    int sms = 0;
+    B2_TRY(device_sm_count(&sms));
+    const int few = kRun == 8 ? sms * (1024 / threads_for(a.width, 1)) : 1024;
+    if (a.width <= 4096 && a.rows <= few) wide(norm_block_kernel<X, T, 1, false, kRun>, 1);
+    else if (a.width <= 1024) launch_pdl(norm_block_kernel<X, T, 4, true, kRun>, dim3(ceil_div(a.rows, 4)), dim3(128), 0, s, a);
     else if (a.width <= 8192) wide(norm_block_kernel<X, T, 2, false, kRun>, 2);
     else if (a.width <= 16384) wide(norm_block_kernel<X, T, 4, false, kRun>, 4);
     else {
