@@ -92,7 +92,7 @@ def build_binding(force: bool = False) -> None:
     part = f"{out}.{os.getpid()}"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{sysconfig.get_paths()['include']}", f"-I{where}/include", "-I/usr/local/cuda/include", src, "-o", part, f"-L{HERE}", "-lb200attn",
-           f"-L{where}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{where}/lib"]
+           f"-L{where}/lib", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{where}/lib"]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
         raise RuntimeError(f"binding build failed: {' '.join(cmd)}\n{p.stderr[-4000:]}")

@@ -4,7 +4,7 @@
 // more rows 14), here 4.8 (6.8, 7.2, 9).  Errors are those of the ctypes binding: its function `fail` raises them.
 #include <Python.h>
 
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -79,7 +79,7 @@ const float* vector(PyObject* o, const char* name, int64_t n) {
     return t.data_ptr<float>();
 }
 
-at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) { return at::empty(size, at::TensorOptions().dtype(type).device(like.device())); }
+at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) { return at::Tensor(at::detail::empty_cuda(size, type, like.device(), std::nullopt)); }
 int64_t codes_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 bool truth(PyObject* o) {
