@@ -260,14 +260,16 @@ int q8_few_rows(const Q8Product& p, cudaStream_t s) {
     plan.units = ceil_div(p.out, 8);
     const int grid = std::max(std::min(plan.units, sms), ceil_div(plan.units * parts, kMostTiles));
     const int tiles = ceil_div(plan.units, grid) * parts;
-    // The split of K with the fewest blocks on the busiest warp; of equal ones that with the fewest slices.
+    // The split of K with the fewest blocks on the busiest warp; of equal ones that with the fewest slices.  Not one whose sums a CTA does not hold: 17 tiles of 8192
+    // columns in 16 slices would want 271 KB.  Unsplit, 64 tiles of 8192 columns take 197 KB with a norm's weights.
+    const auto shared = [&](int slices_log2) { return (size_t)kRows * codes_pitch(p.pitch) + ((size_t)tiles << slices_log2) * 512 + (p.norm_w ? (size_t)p.in * 4 : 0); };
     long long busiest = 0;
     plan.slices_log2 = 0;
-    for (int l = 0; l <= 4; ++l) {
+    for (int l = 0; l <= 4 && (l == 0 || shared(l) <= kMostShared); ++l) {
         const long long blocks = (long long)ceil_div(tiles, kWarps >> l) * ceil_div(chunks, 1 << l);
         if (l == 0 || blocks < busiest) { busiest = blocks; plan.slices_log2 = l; }
     }
-    const size_t smem = (size_t)kRows * codes_pitch(p.pitch) + ((size_t)tiles << plan.slices_log2) * 512 + (p.norm_w ? (size_t)p.in * 4 : 0);
+    const size_t smem = shared(plan.slices_log2);
     if (smem > kMostShared) B2_FAIL(B200ATTN_ERR_UNSUPPORTED, "8-bit product: %zu bytes of shared memory for %d rows of %d columns", smem, p.rows, p.in);
     // More weights than the first fetches of a warp bring in several times over, or long rows of X.  4096 x 2 x 11008 at one row 18.3 us, shallow 21; 1024 x 2 x
     // 3584 at one row 5.4 us, shallow 4.2.

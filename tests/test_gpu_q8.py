@@ -178,6 +178,21 @@ def test_gated(ops, cuda, rows, cols, out, act, y_type):
     assert torch.equal(layer.forward_codes(*ops.quantize_rows(x), out_dtype=y_type), y)
 
 
+@pytest.mark.parametrize("rows,cols,out,gated", [(1, 8192, 14232, False), (16, 6144, 18992, False), (3, 2048, 28456, False), (1, 8192, 14232, True), (16, 1024, 30808, True)])
+def test_few_rows_whose_sums_fill_shared_memory(ops, cuda, rows, cols, out, gated):
+    """One output column tile more than a whole number of warps has, on long rows: the split of K that keeps all warps busy has more sums than a CTA holds."""
+    ws = [rand(s, out, cols, std=1.2 * cols ** -0.5).bfloat16().cuda() for s in (5, 6)[:1 + gated]]
+    x = activations(7, rows, cols, torch.float16)
+    xc, xs = define_codes(x)
+    sums = [product(xc, xs, *define_codes(w)) for w in ws]
+    if gated:
+        y = ops.Int8GatedLinear(*ws, 1).forward(x, out_dtype=torch.float32)
+        judge(y, glu_reference(*sums, 1), glu_bound(*sums, 1, torch.float32), torch.float32)
+    else:
+        y = ops.Int8Linear(ws[0]).forward(x, out_dtype=torch.float32)
+        judge(y, sums[0], PLAIN * sums[0].abs(), torch.float32)
+
+
 @pytest.mark.parametrize("rows", [1, 16, 40, 300])
 @pytest.mark.parametrize("out,pitch", [(1024, 1024), (33, 37), (256, 260)])
 def test_accumulate(ops, cuda, rows, out, pitch):
