@@ -123,7 +123,7 @@ def build_hybrid(config: dict, limits: Limits, shapes: dict):
         raise ValueError("the hybrid stack serves 16-bit weights and activations only")
     return ops.HybridStack(config["num_layers"], config["intermediate_size"], config["vocab_size"], limits.max_seqs, limits.max_seq_len,
                            max(1, (limits.max_pass_rows or limits.max_seq_len) // limits.max_seq_len),
-                           ops.KV_INT8 if config.get("kv_dtype") == "int8" else ops.KV_FP16, int(config.get("int8_weights", 0)),
+                           ops.KV_INT8 if config.get("kv_dtype") == "int8" else ops.KV_FP16, config.get("int8_weights", False),
                            config.get("rms_eps", 1e-6))
 
 

@@ -480,7 +480,8 @@ class Int8Linear:
         self._args = (self.h.value, self.in_features, self.out_features)
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
-        """[rows, in] -> [rows, out] of out_dtype (default: x's), into `out` if given (fp32 and accumulate: added to it)."""
+        """[rows, in] -> [rows, out] of out_dtype (default: x's), into `out` if given (fp32 and accumulate: added to it), which overlaps
+        no input."""
         return (_binding or _native()).forward(*self._args, x, out_dtype, out, accumulate)
 
     def forward_codes(self, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
@@ -623,7 +624,7 @@ class HybridStack(Stack):
     def __init__(self, num_layers=24, intermediate_size=3584, vocab_size=248320, max_seqs=128, max_seq_len=1536,
                  prefill_chunk_seqs=8, kv_dtype=KV_FP16, int8_weights=True, rms_eps=1e-6):
         self.cfg = StackConfig(num_layers, 1024, intermediate_size, vocab_size, max_seqs, max_seq_len, prefill_chunk_seqs,
-                               kv_dtype, int(int8_weights), rms_eps)
+                               kv_dtype, 2 if int8_weights == 2 else 1 if int8_weights else 0, rms_eps)
         self.vocab_size, self.max_seqs = vocab_size, max_seqs
         self.h = C.c_void_p()
         _check(_lib.b200attn_stack_create(C.byref(self.cfg), C.byref(self.h)))

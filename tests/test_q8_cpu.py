@@ -77,3 +77,13 @@ def test_wrappers_want_tensors_of_the_device(ops):
                  lambda: ops.quantize_rows(x.double()), lambda: ops.Int8GatedLinear(x, x, 7)):
         with pytest.raises(ops.InvalidArgument):
             call()
+
+
+@pytest.mark.parametrize("given,held", [(False, 0), (True, 1), (0, 0), (1, 1), (2, 2), (None, 0), (8, 1), ("yes", 1)])
+def test_int8_weights_of_a_stack(ops, monkeypatch, given, held):
+    """Whatever is true asks for 8-bit weights, as ever; 2 for 8-bit products too."""
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: 0
+    monkeypatch.setattr(ops, "_lib", Library())
+    assert ops.HybridStack(1, 64, 64, 1, 16, 1, int8_weights=given).cfg.int8_weights == held
