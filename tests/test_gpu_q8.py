@@ -396,6 +396,88 @@ def test_norm_block_parts(ops, cuda, width):
     assert ((codes.float() * scales[:, None] - typed).abs() <= 0.51 * scales[:, None] + 1e-30).all()
 
 
+PLACES = [(0, 0), (1, 0), (3, 5), (0, 1), (8, 8)]      # values in front of the first row, and behind each
+WIDTHS = [1, 2, 5, 8, 9, 16, 31, 33, 64, 100, 129, 249, 250, 256, 257, 263, 511, 520, 1017, 1024, 1027, 2041, 4089, 4090, 4097, 8185, 8190, 16377, 16380]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset,pad", PLACES)
+def test_quantize_wherever_rows_lie(ops, cuda, dtype, offset, pad):
+    for rows in (1, 3, 37):
+        for cols in WIDTHS:
+            x = activations(rows + cols, rows, cols, dtype, cols + pad, offset)
+            want, s = define_codes(x)
+            for pitch, at in ((cols, 0), (cols + 3, 1), ((cols + 15) // 16 * 16, 0)):
+                codes = torch.full((rows * pitch + at + 16,), 77, dtype=torch.int8, device="cuda")
+                scales = torch.full((rows + 1,), 77.0, device="cuda")
+                assert ops.lib().b200attn_q8_quantize(x.data_ptr(), ops._Q8_DTYPES[dtype], cols + pad, rows, cols, codes[at:].data_ptr(), pitch, scales.data_ptr(),
+                                                      ops._current_stream()) == 0
+                got = codes[at:at + rows * pitch].view(rows, pitch)
+                assert torch.equal(got[:, :cols].cpu().double(), want) and torch.equal(scales[:rows].cpu(), s), (rows, cols, pitch)
+                assert (codes[:at] == 77).all() and (codes[at + rows * pitch:] == 77).all() and (got[:, cols:] == 77).all() and scales[rows] == 77
+
+
+@pytest.mark.parametrize("dtype,x_type", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("offset,pad", PLACES)
+@pytest.mark.parametrize("post,gate", [(False, ""), (True, "token"), (False, "channel")])
+def test_norm_block_wherever_rows_lie(ops, cuda, dtype, x_type, offset, pad, post, gate):
+    """All outputs at once, between values that stay; weights at any multiple of four bytes."""
+    eps, xs, ys = 1e-6, 0.9, 1.5
+    for rows in (1, 3, 37):
+        for width in WIDTHS:
+            pitch = width + pad
+
+            def window(dtype, content=None):
+                buf = torch.full((offset + rows * pitch + 16,), 77.0, dtype=dtype, device="cuda")
+                view = buf[offset:offset + rows * pitch].view(rows, pitch)[:, :width]
+                if content is not None:
+                    view.copy_(content)
+                return buf, view
+            x0, y0, pre, w, g0 = norm_inputs(rows, width, dtype, x_type, post, gate)
+            _, x = window(x_type, x0)
+            _, y = window(dtype, y0)
+            g = window(dtype, g0)[1] if gate == "token" else g0
+            pre = torch.cat([pre[:1], pre])[1:]
+            x_buf, x_out = window(x_type)
+            n_buf, n_out = window(dtype)
+            codes, scales = torch.full((rows + 1, width + 5), 77, dtype=torch.int8, device="cuda"), torch.full((rows + 1,), 77.0, device="cuda")
+            a = ops.NormArgs(rows, width, ops._Q8_DTYPES[dtype], ops._Q8_DTYPES[x_type], x.data_ptr(), pitch)
+            a.d_y, a.ldy, a.x_scale, a.y_scale, a.eps = y.data_ptr(), pitch, xs, ys, eps
+            a.d_post_w, a.d_pre_w = w.data_ptr() if post else None, pre.data_ptr()
+            if gate:
+                a.d_gate, a.ld_gate = g.data_ptr(), pitch if gate == "token" else 0
+            a.d_x_out, a.ldx_out, a.d_out, a.ld_out = x_out.data_ptr(), pitch, n_out.data_ptr(), pitch
+            a.d_codes, a.ld_codes, a.d_scales = codes.data_ptr(), width + 5, scales.data_ptr()
+            assert ops.lib().b200attn_norm_block(C.byref(a), ops._current_stream()) == 0
+            new, e_new, n, e_n, inv, e_inv = norm_reference(x, y, pre, w, g, False, xs, ys, eps)
+            judge(x_out, new, e_new, x_type)
+            judge(n_out, n, e_n, dtype)
+            for buf, view in ((x_buf, x_out), (n_buf, n_out)):
+                assert (buf[:offset] == 77).all() and (buf[offset + rows * pitch:] == 77).all() and (view.as_strided((rows, pad), (pitch, 1), offset + width) == 77).all()
+            assert (codes[rows] == 77).all() and (codes[:, width:] == 77).all() and scales[rows] == 77
+            if post:                          # a code is off by half a step and what 32 bits lose
+                typed = n_out.double()
+                assert ((codes[:rows, :width].double() * scales[:rows, None].double() - typed).abs() <= 0.51 * scales[:rows, None].double() + HALF_STEP[dtype] * typed.abs() + 1e-7).all()
+            else:
+                z = y.cpu().float() * (g.cpu().float() if gate else torch.tensor(1.0))
+                want, s = define_codes((x.cpu().float() * torch.tensor(xs) + z * torch.tensor(ys)) * pre.cpu())
+                assert torch.equal(codes[:rows, :width].cpu().double(), want), (rows, width)
+                ideal = s.double().cuda() * inv[:, 0]
+                judge(scales[:rows], ideal, ideal.abs() * (e_inv[:, 0] + 3 * U), torch.float32)
+
+
+@pytest.mark.parametrize("width", [3, 13, 64, 200, 256, 300])
+def test_norm_block_of_many_short_rows(ops, cuda, width):
+    x, y, pre, post, g = norm_inputs(20011, width, torch.bfloat16, torch.float32, True, "token")
+    new, e_new, n, e_n, _, _ = norm_reference(x, y, pre, post, g, True, 1.0, 1.0, 1e-6)
+    got_x, got_n = ops.norm_block(x, y, pre, post, g, True, out_dtype=torch.bfloat16)
+    judge(got_x, new, e_new, torch.float32)
+    judge(got_n, n, e_n, torch.bfloat16)
+    want, s = define_codes(x)
+    codes, scales = ops.quantize_rows(x)
+    assert torch.equal(codes.cpu().double(), want) and torch.equal(scales.cpu(), s)
+
+
 def test_norm_block_rows_out_of_the_ordinary(ops, cuda):
     x = activations(1, 5, 300, torch.float32)
     clean = ops.norm_block(x, out_dtype=torch.float32)[1]
