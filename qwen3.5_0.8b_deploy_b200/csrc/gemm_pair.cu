@@ -233,13 +233,26 @@ __device__ __forceinline__ void q8_store(const PairArgs& p, const CUtensorMap* m
     }
 }
 
-// first: sums of the columns from col on (gated: of the gate), second: of those 32 further on (gated: of up).  16-bit results go through the fast exponential and
-// division: together they are off by at most 2^-20 of the value where the rounding takes 2^-12.
+// The activation z / (1 + e^-p), p = z (SiLU) or 2 sqrt(2 / pi) (z + 0.044715 z^3) (GELU).  16-bit results: through the fast exponential and division, together off by at
+// most 2^-20 of the value where the rounding takes 2^-12.  fp32 results: e^-p = 2^(t + r), t + r = -p log2(e) with log2(e) in two parts, 2^t from the library (2^-22) and
+// 2^r = 1 + r ln 2 (|r| < 2^-16, its square nothing), the quotient off by 2^-22.  Below p = -87, where e^-p passes 2^125, the result is z 2^-125 or less as it should be.
+// The library's exponential and a rounded quotient keep the epilogue busy for longer than the products: 17992 x 64 -> 1600 52 us, so 38 (GELU,
+// whose quotients are subnormal more often, 109 and 42), 18 x 232 -> 40 8.5 and 3.4.
+template <typename Y, int kAct>
+__device__ __forceinline__ float q8_activated(float z) {
+    if constexpr (sizeof(Y) == 2) return activated<__nv_bfloat16, kAct>(z);
+    float p = kAct == B200ATTN_ACT_SILU ? z : 1.5957691216057308f * (z + 0.044715f * z * z * z);
+    p = fminf(fmaxf(p, -87.0f), 126.0f);         // a NaN comes back by way of z
+    constexpr float kLog2e = 1.4426950408889634f, kRest = (float)(1.4426950408889634 - (double)kLog2e);
+    const float t = -p * kLog2e, r = fmaf(-p, kRest, fmaf(-p, kLog2e, -t)), e = exp2f(t);
+    return __fdividef(z, 1.0f + fmaf(e, r * 0.6931471805599453f, e));
+}
+
+// first: sums of the columns from col on (gated: of the gate), second: of those 32 further on (gated: of up).
 template <int EPI, typename Y, int kAct, typename Release>
 __device__ __forceinline__ void q8_part(const PairArgs& p, const CUtensorMap* map_y, uint32_t first, uint32_t second, const float* scales, uint32_t stage_smem,
                                         unsigned char* stage, int row, int col, float sx, int lane, Release&& release) {
     constexpr int kCols = 64 / (int)sizeof(Y), kAll = EPI == kPairQ8Glu ? 32 : 64;
-    using A = std::conditional_t<std::is_same<Y, float>::value, float, __nv_bfloat16>;
     uint32_t a[32], b[32];
     tmem_ld32(first, a);
     tmem_ld32(second, b);
@@ -261,7 +274,7 @@ __device__ __forceinline__ void q8_part(const PairArgs& p, const CUtensorMap* ma
                 const float4 u4 = *reinterpret_cast<const float4*>(scales + 32 + c + j);
                 const float u[4] = {u4.x, u4.y, u4.z, u4.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = activated<A, kAct>(v[e]) * value(b[c + j + e], u[e]);
+                for (int e = 0; e < 4; ++e) v[e] = q8_activated<Y, kAct>(v[e]) * value(b[c + j + e], u[e]);
             }
             if constexpr (sizeof(Y) == 4) {
 #pragma unroll
