@@ -9,7 +9,10 @@
 //               rows of the product and the tokens its columns: a thread holds one channel and finds the taps of a token in its own registers.
 //               65536 rows 950 us (projection 878 and convolution 502 before, 3.2 GB between them), 3 x 333 23 (33), 9 x 466 67 (111).
 //
-//   kPairQ8, kPairQ8Glu   products in 8-bit integers, the sums (32-bit integers) times a scale per row and one per column, as they are or gated
+//   kPairQ8, kPairQ8Glu   products in 8-bit integers (kind::i8, slices of 128 columns), the sums (32-bit integers) times a scale per row and one per column, as they
+//               are or gated.  8192 x 4096 -> 4096 bf16 80 us (3.4 POP/s), 65536 x 3584 -> 1024 fp32 170, 8192 x 1024 -> 2 x 3584 fp16 42 (2.9 POP/s; the gate's
+//               exponentials and the stores take as long as the products).  Few slices a tile leave the epilogue as the bound: 8192 x 1024 -> 32768 fp32 300 us
+//               (1.07 GB of results, 161 at the copy rate).
 //
 // A cluster of two CTAs owns a 256 x 256 tile (cta_group::2, M = 256): each CTA fetches its 128 rows of both operands and holds 128 rows of the
 // result, so that an operand byte in shared memory serves twice the products that it would in a tile of one CTA.  Two accumulators of 256 columns

@@ -5,6 +5,9 @@
 // first ones are asked for before the wait on the preceding kernel (weights are complete when b200attn_q8_set_weights returns), so that they arrive while X is
 // quantised.  Each CTA quantises all rows for itself: they are few, and a launch in front would cost more.
 // The sums are 32-bit integers: slices of K meet in shared memory in any order with the same result.
+//
+// 1 x 1024 -> 2 x 3584 fp16 (7.3 MB) 3.5 us, 4.0 with the weights from memory; 16 x 4096 -> 4096 bf16 (16.8 MB) 7.4, of which quantising takes about 3: as a chain of
+// one load, a maximum over the row and one store of codes it is the bound at 16 rows, at one row the chain from launch to the last sums.
 #include "elem.cuh"
 #include "ptx_utils.cuh"
 #include "q8.cuh"

@@ -106,7 +106,7 @@ def product(codes, scale, w_codes, w_scale):
     return (codes.cuda() @ w_codes.cuda().T) * scale.double().cuda()[:, None] * w_scale.double().cuda()[None]
 
 
-def judge(got, want, bound, dtype):
+def within(got, want, bound, dtype):
     """bound: what the steps in 32 bits may be off by; the rounding to dtype comes on top."""
     limit = bound + HALF_STEP[dtype] * (want.abs() + bound) + SMALLEST[dtype]
     err = (got.double() - want).abs()
@@ -155,7 +155,7 @@ def test_linear(ops, cuda, rows, cols, out, x_type, y_type):
     want = product(xc, xs, wc, ws)
     y = layer.forward(x, out_dtype=y_type)
     assert layer.device_status() == 0
-    judge(y, want, PLAIN * want.abs(), y_type)
+    within(y, want, PLAIN * want.abs(), y_type)
     codes, scales = ops.quantize_rows(x)
     again = layer.forward_codes(codes, scales, out_dtype=y_type)
     assert torch.equal(again, y)
@@ -174,7 +174,7 @@ def test_gated(ops, cuda, rows, cols, out, act, y_type):
     g, u = (product(xc, xs, *define_codes(w)) for w in (gate, up))
     y = layer.forward(x, out_dtype=y_type)
     assert layer.device_status() == 0
-    judge(y, glu_reference(g, u, act), glu_bound(g, u, act, y_type), y_type)
+    within(y, glu_reference(g, u, act), glu_bound(g, u, act, y_type), y_type)
     assert torch.equal(layer.forward_codes(*ops.quantize_rows(x), out_dtype=y_type), y)
 
 
@@ -187,10 +187,10 @@ def test_few_rows_whose_sums_fill_shared_memory(ops, cuda, rows, cols, out, gate
     sums = [product(xc, xs, *define_codes(w)) for w in ws]
     if gated:
         y = ops.Int8GatedLinear(*ws, 1).forward(x, out_dtype=torch.float32)
-        judge(y, glu_reference(*sums, 1), glu_bound(*sums, 1, torch.float32), torch.float32)
+        within(y, glu_reference(*sums, 1), glu_bound(*sums, 1, torch.float32), torch.float32)
     else:
         y = ops.Int8Linear(ws[0]).forward(x, out_dtype=torch.float32)
-        judge(y, sums[0], PLAIN * sums[0].abs(), torch.float32)
+        within(y, sums[0], PLAIN * sums[0].abs(), torch.float32)
 
 
 @pytest.mark.parametrize("rows", [1, 16, 40, 300])
@@ -203,7 +203,7 @@ def test_accumulate(ops, cuda, rows, out, pitch):
     layer.forward(x, out=y[:, :out], accumulate=True)
     want = product(*define_codes(x), *define_codes(w))
     total = want + before[:, :out].double()
-    judge(y[:, :out], total, PLAIN * want.abs(), torch.float32)
+    within(y[:, :out], total, PLAIN * want.abs(), torch.float32)
     assert torch.equal(y[:, out:], before[:, out:])
 
 
@@ -248,7 +248,7 @@ def test_largest_sums(ops, cuda):
         x[0] = -1
         want = torch.full((rows, 9), 131072.0, dtype=torch.float64, device="cuda")
         want[0] *= -1
-        judge(ops.Int8Linear(w).forward(x), want, PLAIN * want.abs(), torch.float32)
+        within(ops.Int8Linear(w).forward(x), want, PLAIN * want.abs(), torch.float32)
 
 
 def test_no_rows(ops, cuda):
@@ -348,8 +348,8 @@ def test_norm_block(ops, cuda, rows, width, dtype, x_type, post, gate, xs, ys):
     eps = 1e-6
     new, e_new, n, e_n, _, _ = norm_reference(x, y, pre, post, g, gate == "sigmoid", xs, ys, eps)
     got_x, got_n = ops.norm_block(x, y, pre, post, g, gate == "sigmoid", xs, ys, eps, out_dtype=dtype)
-    judge(got_x, new, e_new, x_type)
-    judge(got_n, n, e_n, dtype)
+    within(got_x, new, e_new, x_type)
+    within(got_n, n, e_n, dtype)
     kept = x.clone()
     again_x, again_n = ops.norm_block(kept, y, pre, post, g, gate == "sigmoid", xs, ys, eps, out_dtype=dtype, in_place=True)
     assert again_x is kept and torch.equal(kept, got_x) and torch.equal(again_n, got_n)
@@ -371,7 +371,7 @@ def test_norm_block_codes(ops, cuda, rows, width, dtype, x_type, gate, xs, ys):
     assert torch.equal(codes.cpu().double(), want)
     _, _, _, _, inv, e_inv = norm_reference(x, y, pre, None, g, False, xs, ys, 1e-6)
     ideal = s.double().cuda() * inv[:, 0]
-    judge(scales, ideal, ideal.abs() * (e_inv[:, 0] + 3 * U), torch.float32)
+    within(scales, ideal, ideal.abs() * (e_inv[:, 0] + 3 * U), torch.float32)
 
 
 @pytest.mark.parametrize("width", [64, 1000, 3000])
@@ -381,9 +381,9 @@ def test_norm_block_parts(ops, cuda, width):
     new, e_new, n, e_n, _, _ = norm_reference(x, None, pre, None, None, False, 1.0, 1.0, 1e-5)
     got_x, got_n = ops.norm_block(x, pre_w=pre, eps=1e-5, out_dtype=torch.float32)
     assert torch.equal(got_x, x)
-    judge(got_n, n, e_n, torch.float32)
+    within(got_n, n, e_n, torch.float32)
     _, _, n, e_n, _, _ = norm_reference(x, y, None, None, None, False, 1.0, 1.0, 1e-6)
-    judge(ops.norm_block(x, y, out_dtype=torch.float32)[1], n, e_n, torch.float32)
+    within(ops.norm_block(x, y, out_dtype=torch.float32)[1], n, e_n, torch.float32)
     a = ops.NormArgs(6, width, ops.DTYPE_F32, ops.DTYPE_F32, x.data_ptr(), width)
     a.d_y, a.ldy, a.x_scale, a.y_scale, a.eps = y.data_ptr(), width, 1.0, 1.0, 1e-6
     keep = torch.full((8, width + 3), 77.0, device="cuda")
@@ -450,8 +450,8 @@ def test_norm_block_wherever_rows_lie(ops, cuda, dtype, x_type, offset, pad, pos
             a.d_codes, a.ld_codes, a.d_scales = codes.data_ptr(), width + 5, scales.data_ptr()
             assert ops.lib().b200attn_norm_block(C.byref(a), ops._current_stream()) == 0
             new, e_new, n, e_n, inv, e_inv = norm_reference(x, y, pre, w, g, False, xs, ys, eps)
-            judge(x_out, new, e_new, x_type)
-            judge(n_out, n, e_n, dtype)
+            within(x_out, new, e_new, x_type)
+            within(n_out, n, e_n, dtype)
             for buf, view in ((x_buf, x_out), (n_buf, n_out)):
                 assert (buf[:offset] == 77).all() and (buf[offset + rows * pitch:] == 77).all() and (view.as_strided((rows, pad), (pitch, 1), offset + width) == 77).all()
             assert (codes[rows] == 77).all() and (codes[:, width:] == 77).all() and scales[rows] == 77
@@ -463,7 +463,7 @@ def test_norm_block_wherever_rows_lie(ops, cuda, dtype, x_type, offset, pad, pos
                 want, s = define_codes((x.cpu().float() * torch.tensor(xs) + z * torch.tensor(ys)) * pre.cpu())
                 assert torch.equal(codes[:rows, :width].cpu().double(), want), (rows, width)
                 ideal = s.double().cuda() * inv[:, 0]
-                judge(scales[:rows], ideal, ideal.abs() * (e_inv[:, 0] + 3 * U), torch.float32)
+                within(scales[:rows], ideal, ideal.abs() * (e_inv[:, 0] + 3 * U), torch.float32)
 
 
 @pytest.mark.parametrize("width", [3, 13, 64, 200, 256, 300])
@@ -471,8 +471,8 @@ def test_norm_block_of_many_short_rows(ops, cuda, width):
     x, y, pre, post, g = norm_inputs(20011, width, torch.bfloat16, torch.float32, True, "token")
     new, e_new, n, e_n, _, _ = norm_reference(x, y, pre, post, g, True, 1.0, 1.0, 1e-6)
     got_x, got_n = ops.norm_block(x, y, pre, post, g, True, out_dtype=torch.bfloat16)
-    judge(got_x, new, e_new, torch.float32)
-    judge(got_n, n, e_n, torch.bfloat16)
+    within(got_x, new, e_new, torch.float32)
+    within(got_n, n, e_n, torch.bfloat16)
     want, s = define_codes(x)
     codes, scales = ops.quantize_rows(x)
     assert torch.equal(codes.cpu().double(), want) and torch.equal(scales.cpu(), s)
@@ -521,7 +521,7 @@ def test_feed_forward(ops, cuda, rows):
     a = act64.abs().amax(1, keepdim=True)
     err = (act64.abs() * 2.0 ** -10 + a / 253.0) @ w.T
     want = h64 + act64 @ (wc * ws.double()[:, None]).cuda().T
-    judge(got, want, err + want.abs() * 8 * U, torch.float32)
+    within(got, want, err + want.abs() * 8 * U, torch.float32)
 
 
 def test_captured_feed_forward_and_another_stream(ops, cuda):
