@@ -566,3 +566,56 @@ def test_weights_given_again(ops, cuda):
     other = big[40:, 100:300]
     ops._check(ops.lib().b200attn_q8_set_weights(layer.h, other.data_ptr(), None, ops.DTYPE_F32, 300, ops._current_stream()))
     assert torch.equal(layer.forward(x), ops.Int8Linear(other.contiguous()).forward(x))
+
+
+# ---- offsets that pass 32 bits -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cols", [4096, 4099])
+def test_rows_far_behind(ops, cuda, cols):
+    """The last rows of matrices of more than 2^31 values, against the same rows by themselves."""
+    rows, last = 2 ** 31 // 4096 + 77, 5
+    x = torch.empty(rows, cols, dtype=torch.float16, device="cuda")
+    x.zero_()
+    x[-last:] = activations(3, last, cols, torch.float16)
+    codes, scales = ops.quantize_rows(x)
+    want, s = ops.quantize_rows(x[-last:].clone())
+    assert torch.equal(codes[-last:], want) and torch.equal(scales[-last:], s) and (scales[:-last] == 0).all()
+    del codes
+    pre, post = (1 + rand(k, cols, std=0.1).cuda() for k in (4, 5))
+    a, b = ops.norm_block(x, x, pre, post, out_dtype=torch.float16)
+    wa, wb = ops.norm_block(x[-last:].clone(), x[-last:].clone(), pre, post, out_dtype=torch.float16)
+    # another split of a row among threads sums its squares in another order: a root mean square off by 208 U of itself at most, so that a result is off by a rounding
+    # of fp16 and what lies below it
+    for got, ref in ((a, wa), (b, wb)):
+        assert ((got[-last:].float() - ref.float()).abs() <= ref.float().abs() * 2.0 ** -10 + 2.0 ** -23).all()
+
+
+@pytest.mark.parametrize("act", [-1, 1])
+@pytest.mark.parametrize("y_type,out", [(torch.float16, 32768), (torch.float32, 32765)])
+def test_results_far_behind(ops, cuda, act, y_type, out):
+    rows, last = 2 ** 31 // 32768 + 300, 5
+    ws = [rand(s, out, 64, std=0.05).cuda() for s in (5, 6)]
+    layer = ops.Int8Linear(ws[0]) if act < 0 else ops.Int8GatedLinear(*ws, act)
+    x = torch.zeros(rows, 64, device="cuda")
+    x[-last:] = activations(3, last, 64, torch.float32)
+    y = layer.forward(x, out_dtype=y_type)
+    want = [product(*define_codes(x[-last:]), *define_codes(w)) for w in ws]
+    if act < 0:
+        within(y[-last:], want[0], PLAIN * want[0].abs(), y_type)
+    else:
+        within(y[-last:], glu_reference(*want, act), glu_bound(*want, act, y_type), y_type)
+    assert not y[:-last].any() and layer.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_weights_far_behind(ops, cuda, rows):
+    """More than 2^31 codes: the last columns against a layer of them alone."""
+    out, last = 2 ** 31 // 8192 + 100, 64
+    w = torch.zeros(out, 8192, dtype=torch.bfloat16, device="cuda")
+    w[-last:] = rand(5, last, 8192, std=0.02).bfloat16().cuda()
+    layer = ops.Int8Linear(w)
+    x = activations(7, rows, 8192, torch.float16)
+    y = layer.forward(x, out_dtype=torch.float32)
+    assert torch.equal(y[:, -last:], ops.Int8Linear(w[-last:]).forward(x, out_dtype=torch.float32)) and not y[:, :-last].any()
+    codes, scales = layer.weight_codes()
+    want, s = define_codes(w[-last:])
+    assert torch.equal(codes[-last:].cpu().double(), want) and torch.equal(scales[-last:].cpu(), s)
