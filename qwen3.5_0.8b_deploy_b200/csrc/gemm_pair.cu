@@ -30,7 +30,6 @@ namespace b200 {
 namespace {
 
 constexpr uint32_t kOperand = 128 * 128;                // 128 rows of 64 two-byte elements
-constexpr uint32_t kStage = 2 * kOperand;
 constexpr int kEpiWarps = 16;
 constexpr int kThreads = 32 * (kEpiWarps + 2);          // epilogue warps, one for loads, one for TMEM and (CTA 0) the products
 
@@ -39,9 +38,12 @@ constexpr bool is_q8(int epi) { return epi == kPairQ8 || epi == kPairQ8Glu; }
 constexpr int kConvTokens = 253;                        // of a tile of 256 columns: the first three are the taps of the fourth
 constexpr int kMaxSeqRows = 512;                        // first rows and slots of the sequences kept in shared memory, up to so many sequences
 
-template <int EPI>
+// kNarrow: all parts are 64 columns wide, so that a slice takes 20 KB and eight of them fit where five do (64 x 8192 -> 1024 10.8 us, with five 11.3; 32 x 3584 ->
+// 1024 6.6 and 6.8).
+template <int EPI, bool kNarrow>
 struct PairSmem {
-    static constexpr int kStages = EPI == kPairConv || is_q8(EPI) ? 5 : 6; // ring of 128-byte slices, 32 KB each per CTA
+    static constexpr int kStages = kNarrow ? 8 : EPI == kPairConv || is_q8(EPI) ? 5 : 6;      // ring of 128-byte slices
+    static constexpr uint32_t kStage = kNarrow ? kOperand + 32 * 128 : 2 * kOperand;
     static constexpr uint32_t kOut = kStages * kStage;                     // 2 KB per epilogue warp
     static constexpr uint32_t kExtra = kOut + kEpiWarps * 2048;            // kPairConv: the tables of conv_part, 8-bit products: 64 scales per epilogue warp
     static constexpr uint32_t kBars = kExtra + (EPI == kPairConv ? 4096 + 4096 + 2048 + 8 * kMaxSeqRows : is_q8(EPI) ? kEpiWarps * 256 : 0);
@@ -506,12 +508,12 @@ __device__ __forceinline__ void conv_part(const LaConvArgs& a, const PairMaps& m
 // grid 2 x pairs, clusters of two.  Rank 0 of a pair issues the products once its own slice and its neighbour's have landed: the copies of both CTAs
 // complete on its barrier.  Every barrier here is signalled from the other CTA too, so all waits are of cluster scope.  Operand a gives the rows of
 // the product (X, kPairConv: W), b its columns.
-template <int EPI, typename T, int kAct>
+template <int EPI, typename T, int kAct, bool kNarrow>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
-    using Smem = PairSmem<EPI>;
+    using Smem = PairSmem<EPI, kNarrow>;
     constexpr int kStages = Smem::kStages;
-    constexpr uint32_t kBars = Smem::kBars;
+    constexpr uint32_t kStage = Smem::kStage, kBars = Smem::kBars;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -584,7 +586,7 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
                     if (rank == 0) mbar_arrive_expect_tx(full(s), bytes);          // the neighbour's bytes may come in first: the phase waits for this arrival
                     tma_load_2d_pair(dst, &maps.a, bar, k, a_row);
                     if constexpr (is_q8(EPI)) {                                    // W in blocks of 8 rows x 128 columns
-                        if (w.width == 256) tma_load_4d_pair(dst + kOperand, &maps.b, bar, 0, 0, k / 128, b_row / 8);
+                        if (!kNarrow && w.width == 256) tma_load_4d_pair(dst + kOperand, &maps.b, bar, 0, 0, k / 128, b_row / 8);
                         else
                             for (int r = 0; r < w.width / 2; r += 32) tma_load_4d_pair(dst + kOperand + r * 128, &maps.b32, bar, 0, 0, k / 128, (b_row + r) / 8);
                     } else if (w.width == 256) tma_load_2d_pair(dst + kOperand, &maps.b, bar, k, b_row);
@@ -743,21 +745,25 @@ gemm_pair_kernel(const __grid_constant__ PairMaps maps, const PairArgs p) {
     if (threadIdx.x == 0 && *abort_flag) atomicExch(p.error, 7);
 }
 
-template <int EPI, typename T, int kAct>
+template <int EPI, typename T, int kAct, bool kNarrow = false>
 int launch_pair(const PairMaps& maps, PairArgs p, cudaStream_t s) {
-    static PerDeviceOnce once;
-    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(gemm_pair_kernel<EPI, T, kAct>, cudaFuncAttributeMaxDynamicSharedMemorySize, PairSmem<EPI>::kBytes)));
     int sms = 0;
     B2_TRY(device_sm_count(&sms));
-    cudaLaunchConfig_t cfg = {};
     // Whole rounds of tiles, then the rest in parts as narrow as it takes to give every pair one (at least 64 columns).
     const int tiles = p.row_tiles * p.col_tiles, pairs = sms / 2, rest = tiles % pairs;
     p.split_log2 = rest == 0 || EPI == kPairConv ? 0 : rest * 4 <= pairs ? 2 : rest * 2 <= pairs ? 1 : 0;
     p.whole = tiles - rest;
     p.items = p.whole + (rest << p.split_log2);
+    if constexpr (is_q8(EPI) && !kNarrow) {
+        if (p.whole == 0 && p.split_log2 == 2) return launch_pair<EPI, T, kAct, true>(maps, p, s);
+    }
+    constexpr uint32_t kBytes = PairSmem<EPI, kNarrow>::kBytes;
+    static PerDeviceOnce once;
+    B2_PER_DEVICE_ONCE(once, B2_CUDA(cudaFuncSetAttribute(gemm_pair_kernel<EPI, T, kAct, kNarrow>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes)));
+    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * std::min(p.items, pairs));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = PairSmem<EPI>::kBytes;
+    cfg.dynamicSmemBytes = kBytes;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -766,7 +772,7 @@ int launch_pair(const PairMaps& maps, PairArgs p, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = g_flags.pdl ? 2 : 1;
-    B2_CUDA(cudaLaunchKernelEx(&cfg, gemm_pair_kernel<EPI, T, kAct>, maps, p));
+    B2_CUDA(cudaLaunchKernelEx(&cfg, gemm_pair_kernel<EPI, T, kAct, kNarrow>, maps, p));
     count_launch();
     return 0;
 }
