@@ -252,19 +252,20 @@ __device__ __forceinline__ void q8_store(const PairArgs& p, const CUtensorMap* m
     }
 }
 
-// The activation z / (1 + e^-p), p = z (SiLU) or 2 sqrt(2 / pi) (z + 0.044715 z^3) (GELU).  16-bit results: through the fast exponential and division, together off by at
-// most 2^-20 of the value where the rounding takes 2^-12.  fp32 results: e^-p = 2^(t + r), t + r = -p log2(e) with log2(e) in two parts, 2^t from the library (2^-22) and
-// 2^r = 1 + r ln 2 (|r| < 2^-16, its square nothing), the quotient off by 2^-22.  Below p = -87, where e^-p passes 2^125, the result is z 2^-125 or less as it should be.
-// The library's exponential and a rounded quotient keep the epilogue busy for longer than the products: 17992 x 64 -> 1600 52 us, so 38 (GELU,
-// whose quotients are subnormal more often, 109 and 42), 18 x 232 -> 40 8.5 and 3.4.
+// The activation z / (1 + e^-p), p = z (SiLU) or 2 sqrt(2 / pi) (z + 0.044715 z^3) (GELU).  16-bit results: through the fast exponential, off by 2^-22 + 1.18 |p| 2^-23 of itself
+// (|p| is 87 at most where the result is not zero: 2^-16), and the fast division (2^-22), where the rounding takes 2^-12 (fp16) or 2^-9.  fp32 results: with w = e^-|p|, which cannot
+// overflow, z w / (1 + w) for negative p and z / (1 + w) for the others.  w = 2^(t + r), t + r = -|p| log2(e) with log2(e) in two parts, 2^t from the library (2^-22) and
+// 2^r = 1 + r ln 2 (|r| < 2^-16, its square nothing), the quotient off by 2^-22.  From |p| = 104 on w is zero, and with it what a negative z gives (NaN for minus infinity, as in
+// the formula).  The library's exponential and a rounded quotient keep the epilogue busy for longer than the products: 17992 x 64 -> 1600 52 us, so 37 (GELU,
+// whose quotients are subnormal more often, 109 and 41), 18 x 232 -> 40 8.5 and 3.5.
 template <typename Y, int kAct>
 __device__ __forceinline__ float q8_activated(float z) {
     if constexpr (sizeof(Y) == 2) return activated<__nv_bfloat16, kAct>(z);
-    float p = kAct == B200ATTN_ACT_SILU ? z : 1.5957691216057308f * (z + 0.044715f * z * z * z);
-    p = fminf(fmaxf(p, -87.0f), 126.0f);         // a NaN comes back by way of z
+    const float p = kAct == B200ATTN_ACT_SILU ? z : 1.5957691216057308f * (z + 0.044715f * z * z * z);
     constexpr float kLog2e = 1.4426950408889634f, kRest = (float)(1.4426950408889634 - (double)kLog2e);
-    const float t = -p * kLog2e, r = fmaf(-p, kRest, fmaf(-p, kLog2e, -t)), e = exp2f(t);
-    return __fdividef(z, 1.0f + fmaf(e, r * 0.6931471805599453f, e));
+    const float a = fminf(fabsf(p), 126.0f);     // a NaN comes back by way of z
+    const float t = -a * kLog2e, r = fmaf(-a, kRest, fmaf(-a, kLog2e, -t)), e = exp2f(t), w = fmaf(e, r * 0.6931471805599453f, e);
+    return __fdividef(p < 0.0f ? z * w : z, 1.0f + w);
 }
 
 // first: sums of the columns from col on (gated: of the gate), second: of those 32 further on (gated: of up).
