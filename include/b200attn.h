@@ -495,7 +495,7 @@ int b200attn_stack_residual(b200attn_stack st, int rows, float* d_out, int stop_
  * ---------------------------------------------------------------------------------------------- */
 typedef struct b200attn_q8_s* b200attn_q8;   /* weights of an 8-bit product; read-only between calls of set_weights, so that streams may share it */
 
-/* Codes [rows, ld_codes] and scales [rows] of x [rows, cols].  The reference quantises weights this way, in place and by output channel
+/* Codes [rows, ld_codes] and scales [rows] of x [rows, cols], cols <= 2^31 - 1024 (rows of every operator likewise).  The reference quantises weights this way, in place and by output channel
  * (src/backend/cuda/kernels/mlp_cuda.cu:22-39); it has no counterpart for activations. */
 int b200attn_q8_quantize(const void* d_x, int dtype, long long ldx, int rows, int cols, int8_t* d_codes, long long ld_codes, float* d_scales,
                          b200attn_stream stream);

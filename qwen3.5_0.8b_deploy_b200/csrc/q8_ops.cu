@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kMostIn = 131072;              // 127 * 127 * in < 2^31
 constexpr int kMostRows = INT_MAX - 1023;     // rounded up to whole tiles they are still ints
+constexpr int kMostCols = INT_MAX - 1023;     // of the quantiser, whose threads walk a row by steps of up to 512: the first column behind it is still an int
 constexpr int kPitchStep = 128;              // a slice of the products
 
 bool elem_of(int dtype, ElemType* t) {
@@ -89,7 +90,7 @@ extern "C" int b200attn_q8_quantize(const void* d_x, int dtype, long long ldx, i
                                     b200attn_stream stream) {
     ElemType t;
     B2_CHECK_ARG(elem_of(dtype, &t), "q8_quantize: bad element type %d", dtype);
-    B2_CHECK_ARG(rows >= 0 && rows <= kMostRows && cols > 0, "q8_quantize: bad sizes %d x %d", rows, cols);
+    B2_CHECK_ARG(rows >= 0 && rows <= kMostRows && cols > 0 && cols <= kMostCols, "q8_quantize: bad sizes %d x %d", rows, cols);
     B2_CHECK_ARG(ldx >= cols && ld_codes >= cols, "q8_quantize: pitch below %d columns", cols);
     if (rows == 0) return 0;
     B2_CHECK_ARG(d_x && d_codes && d_scales, "q8_quantize: null argument");
