@@ -28,6 +28,7 @@ namespace {
 // behind a boundary, so that they are one access again; weights and codes, which lie otherwise, are turned into place in registers.  What that takes pays for rows above
 // 1024 values: 10000 x 15001 bf16 to codes 90 us, one by one 185; 30000 x 2501 50, 62; but 39816 x 771 24, 22; norms of 5000 x 3001 57, 91; 3000 x 700 8.7, 7.9.
 enum { kSingles = 1, kEights = 8, kShifted = 9 };
+constexpr int kFewestShifted = 1025;             // columns
 template <typename T, bool kWords> struct alignas(16) RawEight { T v[8]; };
 template <> struct alignas(16) RawEight<__half, true> { uint32_t v[4]; };
 template <> struct alignas(16) RawEight<__nv_bfloat16, true> { uint32_t v[4]; };
@@ -537,7 +538,7 @@ struct Rows {
     // others: whether codes and what rows share lie on such boundaries too
     int run(int width, bool others) const {
         if (first == 0 && step == 0 && alike && width % 8 == 0 && others) return kEights;
-        return alike && width > 1024 ? kShifted : kSingles;
+        return alike && width >= kFewestShifted ? kShifted : kSingles;
     }
 };
 template <typename F>
@@ -558,20 +559,28 @@ int quantize(const T* x, long long ldx, int rows, int cols, int8_t* codes, long 
         constexpr int kThreads = decltype(threads)::value;
         launch_pdl(q8_quantize_kernel<T, kRun, kThreads, decltype(groups)::value, kBlocks>, dim3(blocks_for<kThreads>(rows)), dim3(block), 0, s, x, ldx, rows, cols, codes, ldc, scales);
     };
+    const std::integral_constant<int, 0> any;
     const std::integral_constant<int, kQuantGroups> four;
     const int n = ceil_div(reach(cols, kRun), 8 * kQuantGroups);
+    // The rows of one matrix lie alike, so that those one by one are the short ones: the lanes of a warp hold them.
+    static_assert(32 * 8 * kQuantGroups >= kFewestShifted - 1);
     if (n > kBlockThreads) {
         launch_pdl(q8_quantize_loop_kernel<T, kBlocks>, dim3(rows), dim3(kLoopThreads), 0, s, x, ldx, cols, codes, ldc, scales);
-    } else if (kRun == kEights && n > 32 && n <= 64) {
+    } else if constexpr (kRun == kShifted) {
+        with(any, threads_for(reach(cols, kRun), kQuantGroups), four);
+    } else if (n > 32) {
         // Up to 2048 values a warp holds too: 35484 x 1224 bf16 17.7 us, by blocks of two warps 37.2; 33213 x 2048 28.5 and 35.0.
-        if constexpr (kRun == kEights) with(std::integral_constant<int, 32>{}, kLaneThreads, std::integral_constant<int, 2 * kQuantGroups>{});
-    } else if (kRun != kSingles && n > 32) {
-        with(std::integral_constant<int, kRun != kSingles ? 0 : 32>{}, threads_for(reach(cols, kRun), kQuantGroups), four);
-    } else if constexpr (kRun != kShifted) {
-        if (!kBlocks && n <= 4) with(std::integral_constant<int, kBlocks ? 32 : 4>{}, kLaneThreads, four);
-        else if (!kBlocks && n <= 8) with(std::integral_constant<int, kBlocks ? 32 : 8>{}, kLaneThreads, four);
-        else if (!kBlocks && n <= 16) with(std::integral_constant<int, kBlocks ? 32 : 16>{}, kLaneThreads, four);
-        else if (n <= 32) with(std::integral_constant<int, 32>{}, kLaneThreads, four);
+        if constexpr (kRun == kSingles) B2_FAIL(B200ATTN_ERR_UNSUPPORTED, "q8_quantize: no kernel for %d columns one by one", cols);
+        else if (n <= 64) with(std::integral_constant<int, 32>{}, kLaneThreads, std::integral_constant<int, 2 * kQuantGroups>{});
+        else with(any, threads_for(cols, kQuantGroups), four);
+    } else if (!kBlocks && n <= 4) {
+        with(std::integral_constant<int, kBlocks ? 32 : 4>{}, kLaneThreads, four);
+    } else if (!kBlocks && n <= 8) {
+        with(std::integral_constant<int, kBlocks ? 32 : 8>{}, kLaneThreads, four);
+    } else if (!kBlocks && n <= 16) {
+        with(std::integral_constant<int, kBlocks ? 32 : 16>{}, kLaneThreads, four);
+    } else {
+        with(std::integral_constant<int, 32>{}, kLaneThreads, four);
     }
     B2_LAUNCH_CHECK();
     return 0;
