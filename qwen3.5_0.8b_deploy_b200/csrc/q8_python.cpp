@@ -4,6 +4,7 @@
 // more rows 14), here 4.8 (6.8, 7.2, 9).  Errors are those of the ctypes binding: its function `fail` raises them.
 #include <Python.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -79,6 +80,15 @@ const float* vector(PyObject* o, const char* name, int64_t n) {
     return t.data_ptr<float>();
 }
 
+// Autograd does not see what these calls write: a tensor that requires a gradient is refused as PyTorch refuses leaves, and what was written counts as a new version,
+// so that a graph that has saved the tensor notices.
+void check_writable(const at::Tensor& t, const char* name) {
+    if (at::GradMode::is_enabled() && t.requires_grad()) refuse(std::string(name) + ": requires a gradient and would be written to, which is recorded nowhere");
+}
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, const at::Tensor& like) { return at::Tensor(at::detail::empty_cuda(size, type, like.device(), std::nullopt)); }
 int64_t codes_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
@@ -119,7 +129,10 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // What a product writes to: `out`, or a new matrix of `dtype`.
 Matrix output(const Matrix& x, int64_t features, at::ScalarType dtype, PyObject* out, bool accumulate) {
-    if (out != Py_None) return matrix(tensor(out, "out"), "out", features, x.rows);
+    if (out != Py_None) {
+        check_writable(tensor(out, "out"), "out");
+        return matrix(tensor(out, "out"), "out", features, x.rows);
+    }
     if (accumulate) refuse("accumulate wants an output to add to");
     Matrix y;
     y.code = output_code(dtype);
@@ -130,6 +143,7 @@ Matrix output(const Matrix& x, int64_t features, at::ScalarType dtype, PyObject*
 }
 PyObject* result(PyObject* out, const Matrix& y) {
     if (out == Py_None) return THPVariable_Wrap(y.t);
+    written(y.t);
     Py_INCREF(out);
     return out;
 }
@@ -177,6 +191,7 @@ PyObject* norm_block(PyObject*, PyObject* const* args, Py_ssize_t n) {
     arguments(n, 11);
     const Matrix x = matrix(tensor(args[0], "x"), "x");
     const bool has_y = args[1] != Py_None, in_codes = args[9] == Py_None, in_place = truth(args[10]);
+    if (in_place) check_writable(x.t, "x");
     const at::ScalarType dtype = has_y ? tensor(args[1], "y").scalar_type() : in_codes ? x.t.scalar_type() : type_of(args[9], "out_dtype");
     b200attn_norm_args a{};
     a.dtype = code_of(dtype);
@@ -216,12 +231,14 @@ PyObject* norm_block(PyObject*, PyObject* const* args, Py_ssize_t n) {
         a.ld_codes = pitch;
         a.d_scales = scales.data_ptr<float>();
         check(b200attn_norm_block(&a, stream()));
+        if (in_place) written(x_out);
         return pack({x_out, pitch == x.cols ? codes : codes.narrow(1, 0, x.cols), scales});
     }
     at::Tensor out = empty({x.rows, x.cols}, dtype, x.t);
     a.d_out = out.data_ptr();
     a.ld_out = x.cols;
     check(b200attn_norm_block(&a, stream()));
+    if (in_place) written(x_out);
     return pack({x_out, out});
     END_HANDLE_TH_ERRORS
 }

@@ -404,7 +404,8 @@ class LinearAttention:
 
 # ---- feed-forward in 8-bit integers ------------------------------------------------------------------------------------
 # The calls of a pass (quantize_rows, forward, forward_codes, norm_block) are in csrc/q8_python.cpp, checks of their tensors included: products of a few rows
-# take the GPU 2 to 4 us, less than the same steps take in Python.  They go through the same C ABI.
+# take the GPU 2 to 4 us, less than the same steps take in Python.  They go through the same C ABI.  Nothing here is differentiated: results require no gradient whatever
+# the inputs do.  Where gradients are recorded a tensor that requires one is not written to (out, in_place), and one that is written to gets a new version.
 _binding = None
 
 
@@ -462,7 +463,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 class Int8Linear:
-    """y = x W^T in 8-bit integers: W quantised per output channel when it is given, x per row in every call."""
+    """y = x W^T in 8-bit integers: W quantised per output channel when it is given, x per row in every call.  There is no backward pass: results
+    require no gradient, and an `out` that requires one is refused where gradients are recorded."""
 
     def __init__(self, weight: torch.Tensor):
         self._create([weight], -1)
@@ -525,7 +527,8 @@ def norm_block(x: torch.Tensor, y: torch.Tensor | None = None, pre_w: torch.Tens
     """From one block to the next: x' = x_scale x + y_scale gate(norm(y) post_w), n = norm(x') pre_w.
 
     y is None (no block output yet) or of the activations' type; post_w None leaves its norm out; gate is [rows, width], [width] or None.  Returns
-    (x', n) with n of `out_dtype` (y's type where there is a y), or (x', codes, scales) when out_dtype is None.  in_place: x' is x.
+    (x', n) with n of `out_dtype` (y's type where there is a y), or (x', codes, scales) when out_dtype is None.  in_place: x' is x, which must
+    not require a gradient where gradients are recorded.  There is no backward pass: results require no gradient.
     """
     return (_binding or _native()).norm_block(x, y, pre_w, post_w, gate, sigmoid_gate, x_scale, y_scale, eps, out_dtype, in_place)
 
