@@ -75,10 +75,14 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_binding(force: bool = False) -> None:
-    """_q8.so, the Python calls of the 8-bit operators (csrc/q8_python.cpp): on PyTorch's C++ API, beside the library it calls."""
+    """_q8.so, the Python calls of the 8-bit operators (csrc/q8_python.cpp): on PyTorch's C++ API, beside the library it calls.  C and C++ hosts need neither."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ModuleNotFoundError:
+        print("_q8.so left out: PyTorch is not installed", file=sys.stderr)
+        return
     src, out = os.path.join(CSRC, "q8_python.cpp"), os.path.join(HERE, "_q8.so")
     header = os.path.join(HERE, "..", "include", "b200attn.h")
     # by the interpreter and the PyTorch it was built for too: their interfaces are not the next version's
