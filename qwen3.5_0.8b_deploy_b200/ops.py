@@ -435,9 +435,9 @@ def _invalid(message: str) -> InvalidArgument:
     return InvalidArgument(ERR_INVALID, message)
 
 
-def _matrix(t: torch.Tensor, name: str, cols: int = -1, rows: int = -1, types: dict = _Q8_DTYPES) -> tuple[int, int]:
+def _matrix(t: torch.Tensor, name: str, cols: int = -1, rows: int = -1) -> tuple[int, int]:
     """(type code, row pitch) of a [rows, cols] matrix on the current device whose columns lie side by side; -1: any number."""
-    code, shape = types.get(t.dtype, -1), t.shape
+    code, shape = _Q8_DTYPES.get(t.dtype, -1), t.shape
     if code >= 0 and len(shape) == 2 and t.is_cuda and t.get_device() == _device() and (cols < 0 or shape[1] == cols) and (rows < 0 or shape[0] == rows):
         ld, step = t.stride()
         if shape[0] <= 1:
@@ -482,8 +482,8 @@ class Int8Linear:
         self._args = (self.h.value, self.in_features, self.out_features)
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
-        """[rows, in] -> [rows, out] of out_dtype (default: x's), into `out` if given (fp32 and accumulate: added to it), which overlaps
-        no input."""
+        """[rows, in] -> [rows, out] of out_dtype (default: x's), into `out` if given, whose type then counts (fp32 and accumulate: added to
+        it), and which overlaps no input."""
         return (_binding or _native()).forward(*self._args, x, out_dtype, out, accumulate)
 
     def forward_codes(self, codes: torch.Tensor, scales: torch.Tensor, out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
