@@ -10,7 +10,8 @@
 //   norms on both sides, 49268 x 64, fp32 x      6.5 us from L2 (a warp per row 28.4)
 // What it took beside the single pass: enough warps to cover the loads (norm to codes at 4 / 5 / 6 blocks of four warps an SM: 111.5 / 110.0 / 119.9 us, the last with
 // spills; the second norm at 1 / 2 / 3 blocks: 143 / 127 / 158), no branch on the form of the update inside the eight values of a step (130 us), and a largest value
-// found in packed pairs (the quantiser 115 us without).  Rows of an odd width are bound by their instructions: 30000 x 2501 bf16 to codes 48 us, 34 at the copy rate.
+// found in packed pairs (the quantiser 115 us without).  All in fp32, norm blocks of 520 to 1024 columns spill 80 bytes a thread at five blocks: 65536 x 1024 164 us, with a
+// norm behind the block 171 (164 at the copy rate).  Rows of an odd width are bound by their instructions: 30000 x 2501 bf16 to codes 48 us, 34 at the copy rate.
 #include "elem.cuh"
 #include "ptx_utils.cuh"
 #include "q8.cuh"
@@ -569,7 +570,8 @@ int quantize(const T* x, long long ldx, int rows, int cols, int8_t* codes, long 
     } else if constexpr (kRun == kShifted) {
         with(any, threads_for(reach(cols, kRun), kQuantGroups), four);
     } else if (n > 32) {
-        // Up to 2048 values a warp holds too: 35484 x 1224 bf16 17.7 us, by blocks of two warps 37.2; 33213 x 2048 28.5 and 35.0.
+        // Up to 2048 values a warp holds too: 35484 x 1224 bf16 17.7 us, by blocks of two warps 37.2; 33213 x 2048 28.5 and 35.0;
+        // fp32 32.3 and 38.1; 49.0 and 49.0.
         if constexpr (kRun == kSingles) B2_FAIL(B200ATTN_ERR_UNSUPPORTED, "q8_quantize: no kernel for %d columns one by one", cols);
         else if (n <= 64) with(std::integral_constant<int, 32>{}, kLaneThreads, std::integral_constant<int, 2 * kQuantGroups>{});
         else with(any, threads_for(cols, kQuantGroups), four);
